@@ -1,4 +1,5 @@
-/* Umbrella header: everything the quantized-GEMM drop-in library exports. */
+/* Umbrella header: everything the quantized-GEMM drop-in library exports, and the operators of ext/,
+ * which stand beside it and have no counterpart in the reference's headers. */
 #ifndef KERNEL_SET_H_
 #define KERNEL_SET_H_
 #include "kernel_set/types.h"
@@ -8,4 +9,6 @@
 #include "kernel_set/moe.h"
 #include "kernel_set/activation.h"
 #include "kernel_set/norm.h"
+#include "kernel_set/ext/lora.h"
+#include "kernel_set/ext/moe_backward.h"
 #endif /* KERNEL_SET_H_ */

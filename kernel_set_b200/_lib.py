@@ -226,6 +226,23 @@ _decl("ks_moe_grouped_gemm_fp8_blockwise_masked",
       [_VP, _VP, _VP, POINTER(c_float), POINTER(c_float), POINTER(c_int32), c_int, c_int64, c_int64, c_int64,
        c_int, c_int, c_int, c_int, c_int, _VP])
 
+# ext/moe_backward.h
+_decl("ks_moe_gate_softmax_topk_backward",
+      [_VP, POINTER(c_float), POINTER(c_float), POINTER(c_int32), _VP, c_int64, c_int, c_int, c_int, c_int, _VP])
+_decl("ks_moe_permute_backward", [_VP, _VP, POINTER(c_int32), c_int64, c_int, c_int64, c_int, _VP])
+_decl("ks_moe_unpermute_backward",
+      [_VP, POINTER(c_float), _VP, _VP, POINTER(c_int32), POINTER(c_float), c_int64, c_int, c_int64, c_int, _VP])
+
+# ext/lora.h
+_decl("ks_lora_plan", [POINTER(c_int32), POINTER(c_int32), POINTER(c_int32), c_int64, c_int, _VP])
+_decl("ks_lora_apply",
+      [_VP, c_int64, _VP, c_int64, POINTER(c_float), _VP, c_int64, _VP, _VP, POINTER(c_float), POINTER(c_int32), POINTER(c_int32),
+       c_int64, c_int, c_int, c_int64, c_int64, c_int, _VP])
+_decl("ks_lora_backward_workspace", [POINTER(c_size_t), c_int64, c_int, c_int, c_int64, c_int64])
+_decl("ks_lora_backward",
+      [_VP, c_int64, _VP, _VP, _VP, c_int64, _VP, c_int64, _VP, c_int64, POINTER(c_float), _VP, _VP, POINTER(c_float),
+       POINTER(c_int32), POINTER(c_int32), c_int64, c_int, c_int, c_int64, c_int64, _VP, c_size_t, c_int, _VP])
+
 
 def status_string(status: int) -> str:
     raw = lib.ks_status_string(c_int(status))

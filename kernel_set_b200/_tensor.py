@@ -8,6 +8,7 @@ reference tensor's device (``:205-219``); dtype map ``:81-93``.
 """
 from __future__ import annotations
 
+import contextlib
 from typing import Any, Optional
 
 import torch
@@ -107,6 +108,24 @@ def default_stream(stream: TensorLike, reference: TensorLike = None) -> int:
             return _raw_stream(reference.device.index)
         return torch.cuda.current_stream(reference.device).cuda_stream
     return 0
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device_of(obj: TensorLike):
+    """A context in which the device of ``obj`` is the current one (the library launches on the current device)."""
+    if isinstance(obj, torch.Tensor) and obj.is_cuda and obj.device.index != torch.cuda.current_device():
+        return torch.cuda.device(obj.device)
+    return _HERE
+
+
+def same_dtype(reference: TensorLike, **others: TensorLike) -> None:
+    """Refuses tensors whose type is not ``reference``'s (raw addresses have none)."""
+    if isinstance(reference, torch.Tensor):
+        for name, t in others.items():
+            if isinstance(t, torch.Tensor) and t.dtype != reference.dtype:
+                raise ValueError(f"{name} must be {reference.dtype}, as the other tensors of the call; got {t.dtype}")
 
 
 def infer_dtype(reference: TensorLike, dtype: Optional[int]) -> int:

@@ -42,7 +42,8 @@ def _nvcc() -> str:
 
 def _newest_header() -> float:
     newest = 0.0
-    for base in (CSRC, os.path.join(ROOT, "include", "kernel_set")):
+    include = os.path.join(ROOT, "include", "kernel_set")
+    for base in (CSRC, include, os.path.join(include, "ext")):
         for name in os.listdir(base):
             if name.endswith((".cuh", ".h")):
                 newest = max(newest, os.path.getmtime(os.path.join(base, name)))

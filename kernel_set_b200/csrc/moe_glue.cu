@@ -25,15 +25,13 @@
 #include "common.cuh"
 #include "kernel_set/activation.h"
 #include "kernel_set/moe.h"
+#include "moe_rows.cuh"
 #include "quant_math.cuh"
 #include "sm100_host.cuh"
 #include "sm100_ptx.cuh"
 
 namespace ksb {
 namespace {
-
-constexpr int kMaxExperts = 1024;   // as the reference (moe_gate.cu:33)
-constexpr int kMaxTopK = 32;        // as the reference (moe_gate.cu:35)
 
 // ---------------------------------------------------------------------------------
 // gate: one warp per token
@@ -108,7 +106,14 @@ gate_softmax_topk_kernel(float* __restrict__ out_w, int32_t* __restrict__ out_i,
 constexpr int kPermThreads = 1024;
 constexpr int kPermWarps = kPermThreads / 32;
 
+// The group of an id: itself, or -1 out of range; with REST, out of range and the last group are one.
+template <bool REST>
+__device__ __forceinline__ int group_of(int e, int experts) {
+  return e >= 0 && e < experts ? e : (REST ? experts - 1 : -1);
+}
+
 // Adds the pairs [begin, end) to the warp's row of `cnt`. Loads are issued eight at a time.
+template <bool REST>
 __device__ __forceinline__ void count_pairs(int* mine, const int32_t* __restrict__ topk_idx, int64_t begin,
                                             int64_t end, int experts) {
   for (int64_t base = begin + threadIdx.x; base < end; base += 8 * kPermThreads) {
@@ -116,11 +121,11 @@ __device__ __forceinline__ void count_pairs(int* mine, const int32_t* __restrict
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int64_t i = base + static_cast<int64_t>(j) * kPermThreads;
-      e[j] = i < end ? __ldg(topk_idx + i) : -1;
+      e[j] = i < end ? group_of<REST>(__ldg(topk_idx + i), experts) : -1;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (e[j] >= 0 && e[j] < experts) atomicAdd(mine + e[j], 1);
+      if (e[j] >= 0) atomicAdd(mine + e[j], 1);
   }
 }
 
@@ -139,6 +144,7 @@ __device__ __forceinline__ void fold_counts(int* cnt, int* sum, int experts) {
   __syncthreads();
 }
 
+template <bool REST>
 __global__ void __launch_bounds__(kPermThreads)
 compute_permutation_kernel(int32_t* __restrict__ sorted_ids, int32_t* __restrict__ offsets,
                            const int32_t* __restrict__ topk_idx, int64_t pairs, int experts, int64_t chunk) {
@@ -158,24 +164,24 @@ compute_permutation_kernel(int32_t* __restrict__ sorted_ids, int32_t* __restrict
   const int64_t end = begin + piece < c_end ? begin + piece : c_end;
   const int warps = static_cast<int>((c_end - c_begin + piece - 1) / piece);
   // the ids of a warp's first step stay in registers: with up to 1024 pairs a CTA that is all of them
-  const int e_first = begin + lane < end ? __ldg(topk_idx + begin + lane) : -1;
+  const int e_first = begin + lane < end ? group_of<REST>(__ldg(topk_idx + begin + lane), experts) : -1;
   const int rows = gridDim.x == 1 ? warps : kPermWarps;   // of `cnt` in use
   for (int i = threadIdx.x; i < rows * experts; i += kPermThreads) cnt[i] = 0;
   for (int i = threadIdx.x; i < 2 * experts; i += kPermThreads) before[i] = 0;
   __syncthreads();
   int* mine = cnt + warp * experts;
   if (c_begin > 0) {
-    count_pairs(mine, topk_idx, 0, c_begin, experts);
+    count_pairs<REST>(mine, topk_idx, 0, c_begin, experts);
     fold_counts(cnt, before, experts);
   }
   if (c_end < pairs) {
-    count_pairs(mine, topk_idx, c_end, pairs, experts);
+    count_pairs<REST>(mine, topk_idx, c_end, pairs, experts);
     fold_counts(cnt, total, experts);
   }
   for (int64_t base = begin; base < end; base += 32) {
     const int64_t i = base + lane;
-    const int e = base == begin ? e_first : (i < end ? __ldg(topk_idx + i) : -1);
-    const bool valid = e >= 0 && e < experts;
+    const int e = base == begin ? e_first : (i < end ? group_of<REST>(__ldg(topk_idx + i), experts) : -1);
+    const bool valid = e >= 0;
     const unsigned mask = __match_any_sync(0xffffffffu, valid ? e : experts + lane);
     if (valid && lane == __ffs(mask) - 1) mine[e] += __popc(mask);
     __syncwarp();
@@ -228,8 +234,8 @@ compute_permutation_kernel(int32_t* __restrict__ sorted_ids, int32_t* __restrict
   __syncthreads();
   for (int64_t base = begin; base < end; base += 32) {
     const int64_t i = base + lane;
-    const int e = base == begin ? e_first : (i < end ? __ldg(topk_idx + i) : -1);
-    const bool valid = e >= 0 && e < experts;
+    const int e = base == begin ? e_first : (i < end ? group_of<REST>(__ldg(topk_idx + i), experts) : -1);
+    const bool valid = e >= 0;
     const unsigned mask = __match_any_sync(0xffffffffu, valid ? e : experts + lane);
     if (valid) sorted_ids[total[e] + mine[e] + __popc(mask & ((1u << lane) - 1u))] = static_cast<int32_t>(i);
     __syncwarp();
@@ -311,11 +317,6 @@ inverse_permutation_kernel(int32_t* __restrict__ inverse, const int32_t* __restr
   if (r >= pairs) return;
   const int32_t pair = ids[r];
   if (pair >= 0 && pair < pairs) inverse[pair] = static_cast<int32_t>(r);
-}
-
-// `row` if it is the row of pair `pair`, else -1.
-__device__ __forceinline__ int32_t check_row(int32_t row, const int32_t* __restrict__ ids, int64_t pair, int64_t pairs) {
-  return (row >= 0 && row < pairs && __ldg(ids + row) == pair) ? row : -1;
 }
 
 // Row of a pair after the sort, -1 for a dropped pair. The inverse map of a dropped pair was not
@@ -619,14 +620,48 @@ inline unsigned grid_for(int64_t work_items, int threads = 256) {
   return static_cast<unsigned>(blocks < 1 ? 1 : (blocks < cap ? blocks : cap));
 }
 
-ks_status_t check_pairs(const char* where, int64_t tokens, int top_k, int64_t* pairs) {
-  if (tokens > 0 && top_k > 0 && tokens > INT32_MAX / top_k)
-    KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": num_tokens*top_k exceeds int32 limit");
-  *pairs = tokens * static_cast<int64_t>(top_k);
+}  // namespace
+
+void enqueue_inverse_permutation(int32_t* inverse, const int32_t* ids, int64_t pairs, cudaStream_t stream) {
+  sm100::launch_programmatic(inverse_permutation_kernel, static_cast<unsigned>((pairs + 255) / 256), 256, 0, stream, inverse,
+                             ids, pairs);
+}
+
+ks_status_t enqueue_group_sort(const char* where, int32_t* sorted_ids, int32_t* offsets, const int32_t* ids, int64_t pairs,
+                               int groups, bool rest, cudaStream_t stream) {
+  const size_t smem = (static_cast<size_t>(kPermWarps) + 2) * groups * sizeof(int);
+  // one pair per thread, at most one CTA per SM
+  const int64_t per_cta = (pairs + sm_count() - 1) / sm_count();
+  const int64_t per_thread = (per_cta + kPermThreads - 1) / kPermThreads;
+  const int64_t chunk = (per_thread > 0 ? per_thread : 1) * kPermThreads;
+  const unsigned ctas = pairs > 0 ? static_cast<unsigned>((pairs + chunk - 1) / chunk) : 1u;
+  // once per device and always: the kernel's static shared memory counts towards the 48 KB that need no
+  // opt-in, so a test of the dynamic part alone left out 361 experts (49096 + 132 bytes)
+  static std::mutex mu;
+  static bool attr_done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+      const int most = static_cast<int>((kPermWarps + 2) * kMaxExperts * sizeof(int));
+      cudaError_t e = cudaFuncSetAttribute(compute_permutation_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(compute_permutation_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (e != cudaSuccess) return cuda_status(e, where);
+      attr_done[dev] = true;
+    }
+  }
+  if (rest)
+    sm100::launch_programmatic(compute_permutation_kernel<true>, ctas, kPermThreads, smem, stream, sorted_ids, offsets, ids,
+                               pairs, groups, chunk);
+  else
+    sm100::launch_programmatic(compute_permutation_kernel<false>, ctas, kPermThreads, smem, stream, sorted_ids, offsets, ids,
+                               pairs, groups, chunk);
+  KSB_CHECK_LAUNCH(where);
   return KS_SUCCESS;
 }
 
-}  // namespace
 }  // namespace ksb
 
 using namespace ksb;
@@ -716,33 +751,7 @@ ks_status_t ks_moe_compute_permutation(int32_t* sorted_token_ids, int32_t* exper
   if (st != KS_SUCCESS) return st;
   st = require_sm100(where);
   if (st != KS_SUCCESS) return st;
-  cudaStream_t s = as_stream(stream);
-  const size_t smem = (static_cast<size_t>(kPermWarps) + 2) * num_experts * sizeof(int);
-  // one pair per thread, at most one CTA per SM
-  const int64_t per_cta = (pairs + sm_count() - 1) / sm_count();
-  const int64_t per_thread = (per_cta + kPermThreads - 1) / kPermThreads;
-  const int64_t chunk = (per_thread > 0 ? per_thread : 1) * kPermThreads;
-  const unsigned ctas = pairs > 0 ? static_cast<unsigned>((pairs + chunk - 1) / chunk) : 1u;
-  // once per device and always: the kernel's static shared memory counts towards the 48 KB that need no
-  // opt-in, so a test of the dynamic part alone left out 361 experts (49096 + 132 bytes)
-  static std::mutex mu;
-  static bool attr_done[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(compute_permutation_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           static_cast<int>((kPermWarps + 2) * kMaxExperts * sizeof(int)));
-      if (e != cudaSuccess) return cuda_status(e, where);
-      attr_done[dev] = true;
-    }
-  }
-  sm100::launch_programmatic(compute_permutation_kernel, ctas, kPermThreads, smem, s,
-      sorted_token_ids, expert_offsets, topk_indices, pairs,
-                                                              num_experts, chunk);
-  KSB_CHECK_LAUNCH(where);
-  return KS_SUCCESS;
+  return enqueue_group_sort(where, sorted_token_ids, expert_offsets, topk_indices, pairs, num_experts, false, as_stream(stream));
 }
 
 ks_status_t ks_moe_permute(void* permuted, const void* input, const int32_t* sorted_token_ids, int64_t num_tokens,

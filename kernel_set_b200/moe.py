@@ -2,7 +2,7 @@
 signatures of ``bindings/python/kernel_set/moe.py`` of the reference project
 (``gate_softmax_topk`` :42-71, ``compute_permutation`` :109-134, ``permute``
 :137-159, ``unpermute`` :162-186, ``grouped_gemm`` :189-217);
-``grouped_gemm_fp8_blockwise`` and ``permute_quant_fp8`` wrap added symbols."""
+``grouped_gemm_fp8_blockwise``, ``permute_quant_fp8`` and the ``*_backward`` wrap added symbols."""
 from __future__ import annotations
 
 from typing import Optional
@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from ._lib import by_address as lib, check
-from ._tensor import TensorLike, default_stream, dtype_to_ks, f32_ptr, i32_ptr, infer_dtype, ptr
+from ._tensor import TensorLike, default_stream, dtype_to_ks, f32_ptr, i32_ptr, infer_dtype, on_device_of, ptr, same_dtype
 
 
 def grouped_gemm(c: TensorLike, a: TensorLike, b: TensorLike, expert_offsets: TensorLike, num_experts: int,
@@ -114,6 +114,52 @@ def unpermute(out: TensorLike, permuted: TensorLike, sorted_token_ids: TensorLik
                                f32_ptr(routing_weights, name="routing_weights"), int(num_tokens), int(top_k),
                                int(hidden), dt, default_stream(stream, permuted)), "ks_moe_unpermute")
     return out
+
+
+def unpermute_backward(d_permuted: TensorLike, d_weights: TensorLike, d_out: TensorLike, permuted: TensorLike,
+                       sorted_token_ids: TensorLike, routing_weights: TensorLike, num_tokens: int, top_k: int, hidden: int,
+                       dtype: Optional[int] = None, stream: TensorLike = None):
+    """Gradient of :func:`unpermute`: ``d_permuted[r] = weight[t,k] * d_out[t]`` for the row ``r`` of pair ``(t, k)`` and
+    ``d_weights[t,k] = <d_out[t], permuted[r]>`` (fp32). Rows without a pair and pairs without a row get zeros; a pair may
+    occur once in ``sorted_token_ids``. ``d_permuted`` may be ``permuted``. Returns ``(d_permuted, d_weights)``."""
+    dt = infer_dtype(permuted, dtype)
+    same_dtype(permuted, d_permuted=d_permuted, d_out=d_out)
+    with on_device_of(permuted):
+        check(lib.ks_moe_unpermute_backward(ptr(d_permuted, name="d_permuted"), f32_ptr(d_weights, name="d_weights"),
+                                            ptr(d_out, name="d_out"), ptr(permuted, name="permuted"),
+                                            i32_ptr(sorted_token_ids, name="sorted_token_ids"),
+                                            f32_ptr(routing_weights, name="routing_weights"), int(num_tokens), int(top_k),
+                                            int(hidden), dt, default_stream(stream, permuted)), "ks_moe_unpermute_backward")
+    return d_permuted, d_weights
+
+
+def permute_backward(d_input: TensorLike, d_permuted: TensorLike, sorted_token_ids: TensorLike, num_tokens: int, top_k: int,
+                     hidden: int, dtype: Optional[int] = None, stream: TensorLike = None) -> TensorLike:
+    """Gradient of :func:`permute`: ``d_input[t]`` is the sum of token ``t``'s rows of ``d_permuted``, in slot order, in
+    fp32; a pair may occur once in ``sorted_token_ids``."""
+    dt = infer_dtype(d_permuted, dtype)
+    same_dtype(d_permuted, d_input=d_input)
+    with on_device_of(d_permuted):
+        check(lib.ks_moe_permute_backward(ptr(d_input, name="d_input"), ptr(d_permuted, name="d_permuted"),
+                                          i32_ptr(sorted_token_ids, name="sorted_token_ids"), int(num_tokens), int(top_k),
+                                          int(hidden), dt, default_stream(stream, d_permuted)), "ks_moe_permute_backward")
+    return d_input
+
+
+def gate_softmax_topk_backward(d_logits: TensorLike, d_weights: TensorLike, weights: TensorLike, indices: TensorLike,
+                               logits: TensorLike, num_tokens: int, num_experts: int, top_k: int, renormalize: bool = True,
+                               dtype: Optional[int] = None, stream: TensorLike = None) -> TensorLike:
+    """Gradient of :func:`gate_softmax_topk` with respect to the logits. ``weights`` and ``indices`` are what the gate
+    gave; ``logits`` may be ``None`` with ``renormalize``. ``d_logits`` may be ``logits``."""
+    dt = infer_dtype(d_logits, dtype)
+    same_dtype(d_logits, logits=logits)
+    with on_device_of(d_logits):
+        check(lib.ks_moe_gate_softmax_topk_backward(ptr(d_logits, name="d_logits"), f32_ptr(d_weights, name="d_weights"),
+                                                    f32_ptr(weights, name="weights"), i32_ptr(indices, name="indices"),
+                                                    ptr(logits, name="logits"), int(num_tokens), int(num_experts), int(top_k),
+                                                    1 if renormalize else 0, dt, default_stream(stream, d_logits)),
+              "ks_moe_gate_softmax_topk_backward")
+    return d_logits
 
 
 def grouped_gemm_fp8_blockwise_masked(out: TensorLike, a_fp8: TensorLike, b_fp8: TensorLike, a_scale: TensorLike,
