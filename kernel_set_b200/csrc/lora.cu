@@ -10,6 +10,7 @@
 #include "lora_math.cuh"
 #include "moe_rows.cuh"
 #include "sm100_host.cuh"
+#include "sm100_lora.cuh"
 #include "sm100_ptx.cuh"
 
 namespace ksb {
@@ -84,7 +85,8 @@ __global__ void __launch_bounds__(kAnyThreads) lora_weight_grad_any_kernel(LoraW
   }
 }
 
-ks_status_t run_pass(const char* where, const LoraPass& p, ks_dtype_t dtype, cudaStream_t s) {
+ks_status_t run_pass(const char* where, const LoraPass& p, bool forward, ks_dtype_t dtype, cudaStream_t s) {
+  if (sm100::lora_tile_takes(p)) return sm100::lora_tile_pass(where, p, forward, dtype, s);
   const unsigned grid = static_cast<unsigned>(p.rows);
   const size_t smem = static_cast<size_t>(p.rank) * sizeof(float);
   if (dtype == KS_DTYPE_F16) sm100::launch_programmatic(lora_any_kernel<__half>, grid, kAnyThreads, smem, s, p);
@@ -163,6 +165,8 @@ ks_status_t ks_lora_apply(void* out, int64_t ld_out, const void* base, int64_t l
   if (out == x) KSB_FAIL(KS_ERROR_INVALID_ARGUMENT, "ks_lora_apply: out must not be x");
   st = require_sm100(where);
   if (st != KS_SUCCESS) return st;
+  st = poll_kernel_fault(where);
+  if (st != KS_SUCCESS) return st;
   LoraPass p = {};
   p.out = out; p.base = base; p.in = x; p.u = a; p.v = b; p.scales = scales; p.ids = sorted_ids; p.offsets = offsets;
   p.inner = h;
@@ -170,7 +174,7 @@ ks_status_t ks_lora_apply(void* out, int64_t ld_out, const void* base, int64_t l
   p.rows = num_tokens; p.d_in = k; p.d_out = n;
   p.u_j = k; p.u_i = 1; p.v_o = rank; p.v_j = 1;
   p.adapters = num_adapters; p.rank = rank; p.scale_inner = false;
-  return run_pass(where, p, dtype, as_stream(stream));
+  return run_pass(where, p, true, dtype, as_stream(stream));
 }
 
 ks_status_t ks_lora_backward_workspace(size_t* bytes, int64_t num_tokens, int num_adapters, int rank, int64_t k, int64_t n) {
@@ -213,6 +217,8 @@ ks_status_t ks_lora_backward(void* d_x, int64_t ld_d_x, void* d_a, void* d_b, co
     KSB_FAIL(KS_ERROR_INVALID_ARGUMENT, "ks_lora_backward: workspace missing, too small or not 16-byte aligned");
   st = require_sm100(where);
   if (st != KS_SUCCESS) return st;
+  st = poll_kernel_fault(where);
+  if (st != KS_SUCCESS) return st;
   cudaStream_t s = as_stream(stream);
   float* g = static_cast<float*>(workspace);
   if (num_tokens > 0) {
@@ -223,7 +229,7 @@ ks_status_t ks_lora_backward(void* d_x, int64_t ld_d_x, void* d_a, void* d_b, co
     p.rows = num_tokens; p.d_in = n; p.d_out = k;
     p.u_j = 1; p.u_i = rank; p.v_o = 1; p.v_j = k;
     p.adapters = num_adapters; p.rank = rank; p.scale_inner = true;
-    st = run_pass(where, p, dtype, s);
+    st = run_pass(where, p, false, dtype, s);
     if (st != KS_SUCCESS) return st;
   }
   LoraWeightGrad w = {};

@@ -1,0 +1,583 @@
+// Low-rank adapters on the tensor cores: y = y0 + s V (U x) for rows sorted by adapter, forward and, with the factors'
+// roles changed, the gradient of the input.
+//
+// A tile is up to 128 rows of one adapter, and one cluster of CTAs does both products of it: each CTA multiplies its slice
+// of U's columns with the rows' elements there, the partial sums [128 x rank] are added up over distributed shared memory
+// (every CTA adds all of them, in rank order, so all hold the same bits), and each CTA gives its slice of the outputs. The
+// inner vectors never leave the SM, there is one launch, and while the partial sums are exchanged the rows of y0 and V's
+// tiles are already on their way: both phases draw on one ring of shared-memory stages.
+//   warps 0-3   epilogue: a thread per row. Partial sums out of tensor memory, exchange, split into two 16-bit numbers,
+//               back into tensor memory as the second product's A operand; then y0 + c D, in the stage that holds y0's tile,
+//               and out in whole 128-byte row segments
+//   warps 4-7   producer: cp.async of 16 bytes. Rows are gathered by number, tails come as zeros, and neither
+//               needs a tensor map (the smallest calls are bound by the host's path)
+//   warp 8      tcgen05.mma: M 128 (rows) x N rank, then M 128 x N 64 (outputs) with K = rank, twice (high and low part)
+// Bound by memory: rows * (d_in + 2 d_out) elements are moved, 2 rank operations for each; the legacy tensor path would be the bound
+// from rank 32 on.
+#include <algorithm>
+#include <mutex>
+#include <string>
+
+#include "sm100_lora.cuh"
+#include "sm100_host.cuh"
+#include "sm100_ptx.cuh"
+
+namespace ksb {
+namespace sm100 {
+namespace {
+
+constexpr int kTile = kLoraTile;
+constexpr int kChunk = 64;                         // columns of a stage: 128 bytes
+constexpr int kRowsBytes = kTile * kChunk * 2;     // rows' part of a stage
+constexpr int kBlockBytes = 64 * kChunk * 2;       // 64 rows x 128 bytes of a factor
+constexpr int kEpiWarps = 4, kProdWarps = 4;
+constexpr int kProdThreads = kProdWarps * 32;
+constexpr int kThreads = (kEpiWarps + kProdWarps + 1) * 32;
+constexpr int kMaxCluster = 8;
+
+// RB: 64-rank blocks (rank <= 64 RB).
+template <int RB>
+struct TileCfg {
+  static constexpr int kStages = RB == 1 ? 3 : 4;
+  static constexpr int kLag = kStages - 1;          // stages whose copies are in flight behind the one being issued
+  static constexpr int kStageBytes = kRowsBytes + RB * kBlockBytes;
+  static constexpr int kExchange = kTile * 64 * RB * 4;
+  static constexpr int kLo = 64 * RB;               // tensor memory: sums / high part, low part, two output buffers
+  static constexpr int kOut = kLo + 32 * RB;
+  static constexpr int kTmemCols = RB == 1 ? 256 : 512;
+  static constexpr int kPerSm = RB == 1 ? 2 : 1;
+  static_assert(kOut + 2 * kChunk <= kTmemCols, "tensor memory layout");
+  static constexpr int kBars = 3 * kStages + 7;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + kExchange + kTile * 4 + 8 * kBars + 64;
+  static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory");
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// What this thread's copies (or stores) wrote to shared memory, for the tensor cores to read.
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Arrives on the barrier at the same place in the cluster's CTA `rank`; orders this thread's earlier writes.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, uint32_t rank) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_map_shared(bar, rank)) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_cluster(const WaitCtx& ctx, uint32_t bar, uint32_t parity, uint32_t code) {
+  const auto done = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+  const unsigned long long t0 = global_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (done()) return true;
+    if (ctx.raised()) return false;
+    if (global_ns() - t0 > kWaitLimitNs) {
+      ctx.give_up(code);
+      return false;
+    }
+  }
+}
+// Lane i of the warp writes 8 consecutive columns of tensor memory lane (taddr.lane + i).
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+template <typename T>
+struct Pair;   // two 16-bit numbers in a word
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+};
+
+// The power of two 2^-e for a row whose largest magnitude is `most`, so that most 2^-e is in [1, 2) where possible, and 2^e.
+// It keeps what f16 could not hold (sums beyond 65504, small ones whose low part would vanish) exact; 1 for zeros and non-finite rows.
+__device__ __forceinline__ void row_scale(float most, float* down, float* up) {
+  uint32_t e = (__float_as_uint(most) >> 23) & 255u;
+  if (e == 0u || e == 255u) e = 127u;
+  e = e > 253u ? 253u : e;
+  *down = __uint_as_float((254u - e) << 23);
+  *up = __uint_as_float(e << 23);
+}
+
+struct TileParams {
+  LoraPass p;
+  unsigned int* fault_word;
+  uint32_t idesc1, idesc2;
+  int rank16;       // rank rounded up to 16
+  int cluster;
+};
+
+// Where tile `index` lies: adapter (`adapters` for the rows without one, -1 past the last tile), first place and row count.
+struct TilePlace {
+  int adapter;
+  int count;
+  int64_t place;
+};
+
+// Found by one warp: a lane counts the tiles of a run of adapters, the one whose run holds the tile walks it again.
+__device__ __forceinline__ TilePlace find_tile(const int32_t* __restrict__ offsets, int adapters, int64_t rows, int64_t index) {
+  const int lane = threadIdx.x & 31;
+  const int groups = adapters + 1;
+  const int run = (groups + 31) / 32;
+  const int first = lane * run < groups ? lane * run : groups;
+  const int last = first + run < groups ? first + run : groups;
+  const auto begin_of = [&](int g) { return g > adapters ? rows : lora_offset(offsets, g, rows); };
+  int64_t mine = 0;
+#pragma unroll 4
+  for (int g = first; g < last; ++g) {
+    const int64_t n = begin_of(g + 1) - begin_of(g);
+    mine += n > 0 ? (n + kTile - 1) / kTile : 0;
+  }
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  TilePlace f{-1, 0, 0};
+  const bool here = index < upto && index >= upto - mine;
+  if (here) {
+    int64_t left = index - (upto - mine);
+    for (int g = first; g < last; ++g) {
+      const int64_t b = begin_of(g), n = begin_of(g + 1) - b;
+      const int64_t tiles = n > 0 ? (n + kTile - 1) / kTile : 0;
+      if (left < tiles) {
+        f.adapter = g;
+        f.place = b + left * kTile;
+        const int64_t rest = n - left * kTile;
+        f.count = static_cast<int>(rest < kTile ? rest : kTile);
+        break;
+      }
+      left -= tiles;
+    }
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, here);
+  if (who == 0u) return f;
+  const int src = __ffs(who) - 1;
+  f.adapter = __shfl_sync(0xffffffffu, f.adapter, src);
+  f.count = __shfl_sync(0xffffffffu, f.count, src);
+  f.place = __shfl_sync(0xffffffffu, f.place, src);
+  return f;
+}
+
+template <typename T, int RB, bool FWD>
+__global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kernel(const __grid_constant__ TileParams q) {
+  using C = TileCfg<RB>;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const LoraPass& p = q.p;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t ring = smem_u32(smem);
+  const uint32_t exchange = ring + C::kStages * C::kStageBytes;
+  int32_t* row_of = reinterpret_cast<int32_t*>(smem + C::kStages * C::kStageBytes + C::kExchange);
+  uint64_t* bar_mem = reinterpret_cast<uint64_t*>(row_of + kTile);
+  const uint32_t bars = smem_u32(bar_mem);
+  const auto full = [&](int s) { return bars + 8u * s; };                       // copies have landed
+  const auto free1 = [&](int s) { return bars + 8u * (C::kStages + s); };       // first product has read the stage
+  const auto free2 = [&](int s) { return bars + 8u * (2 * C::kStages + s); };   // the epilogue has written it out
+  const uint32_t bar_sums = bars + 8u * (3 * C::kStages);        // first product complete
+  const uint32_t bar_inner = bar_sums + 8;                       // second product's operand is in tensor memory
+  const uint32_t bar_parts = bar_sums + 16;                      // the cluster's partial sums are in shared memory
+  const auto out_full = [&](int b) { return bar_sums + 24u + 8u * b; };
+  const auto out_free = [&](int b) { return bar_sums + 40u + 8u * b; };
+  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(bar_mem + C::kBars);   // tmem address, abort, tile
+  const WaitCtx wctx{smem_u32(const_cast<uint32_t*>(words) + 1), q.fault_word};
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int S = q.cluster;
+  const uint32_t rank = blockIdx.x % S;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full(s), kProdThreads);
+      mbar_init(free1(s), 1);
+      mbar_init(free2(s), kEpiWarps);
+    }
+    mbar_init(bar_sums, 1);
+    mbar_init(bar_inner, kEpiWarps * 32);
+    mbar_init(bar_parts, static_cast<uint32_t>(S) * kEpiWarps);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(out_full(b), 1);
+      mbar_init(out_free(b), kEpiWarps);
+    }
+    words[1] = 0u;
+    fence_barrier_init();
+  }
+  grid_dependency_wait();
+  if (warp == 8) {   // (behind the wait: a kernel that still runs may need the columns)
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(words)), C::kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 0) {
+    const TilePlace f = find_tile(p.offsets, p.adapters, p.rows, blockIdx.x / S);
+    if (lane == 0) {
+      words[2] = static_cast<uint32_t>(f.adapter);
+      words[3] = static_cast<uint32_t>(f.count);
+    }
+    for (int i = lane; i < kTile; i += 32) row_of[i] = i < f.count ? static_cast<int32_t>(lora_row(p.ids, f.place + i, p.rows)) : -1;
+  }
+  tc_fence_before_sync();
+  if (S > 1) cluster_sync();   // (the barriers that other CTAs arrive on are initialised)
+  else __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = words[0];
+  const int adapter = static_cast<int>(words[2]);
+  const int count = static_cast<int>(words[3]);
+
+  // this CTA's 64-column chunks of the inputs and of the outputs
+  const int in_chunks = static_cast<int>((p.d_in + kChunk - 1) / kChunk), out_chunks = static_cast<int>((p.d_out + kChunk - 1) / kChunk);
+  const int in0 = static_cast<int>(static_cast<int64_t>(in_chunks) * rank / S);
+  const int n1 = static_cast<int>(static_cast<int64_t>(in_chunks) * (rank + 1) / S) - in0;
+  const int out0 = static_cast<int>(static_cast<int64_t>(out_chunks) * rank / S);
+  const int n2 = static_cast<int>(static_cast<int64_t>(out_chunks) * (rank + 1) / S) - out0;
+
+  if (adapter == p.adapters) {
+    // rows without an adapter: y = y0
+    if (p.out != p.base) {
+      const int64_t c0 = static_cast<int64_t>(out0) * kChunk;
+      const int64_t c1 = min(p.d_out, c0 + static_cast<int64_t>(n2) * kChunk);
+      for (int r = warp; r < count; r += kThreads / 32) {
+        const int64_t row = row_of[r];
+        if (row < 0) continue;
+        const T* src = static_cast<const T*>(p.base) + row * p.ld_base;
+        T* dst = static_cast<T*>(p.out) + row * p.ld_out;
+        for (int64_t c = c0 + lane * 8; c < c1; c += 256)
+          *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+      }
+    }
+  } else if (adapter >= 0) {
+    const int total = n1 + n2;
+    if (warp >= 4 && warp < 8) {
+      // ---- producer ----
+      const int t = threadIdx.x - kEpiWarps * 32;
+      const int c8 = t & 7, r0 = t >> 3;
+      const T* u = static_cast<const T*>(p.u) + static_cast<int64_t>(adapter) * p.rank * p.d_in;
+      const T* v = static_cast<const T*>(p.v) + static_cast<int64_t>(adapter) * p.rank * p.d_out;
+      const T* src[8];
+      uint32_t have = 0u;
+      const auto aim = [&](const void* m, int64_t ld) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int32_t row = row_of[r0 + 16 * i];
+          if (row >= 0) have |= 1u << i;
+          src[i] = static_cast<const T*>(m) + (row >= 0 ? row : 0) * ld + c8 * 8;
+        }
+      };
+      aim(p.in, p.ld_in);
+      bool ok = true;
+      const int first2 = n1 % C::kStages;   // stage of the second phase's first chunk
+#pragma unroll 1
+      for (int it = 0; it < total; ++it) {
+        const int s = it % C::kStages;
+        const int before = it - C::kStages;   // the stage's last use
+        if (before >= 0) {
+          if (before < n1) ok = mbar_wait(wctx, free1(s), (before / C::kStages) & 1, 0x31);
+          else ok = mbar_wait(wctx, free2(s), ((before - n1 - (s - first2 + C::kStages) % C::kStages) / C::kStages) & 1, 0x32);
+          if (!ok) break;
+        }
+        if (it == n1) aim(p.base, p.ld_base);
+        const bool one = it < n1;
+        const int64_t col = static_cast<int64_t>(one ? in0 + it : out0 + it - n1) * kChunk;
+        const int64_t width = one ? p.d_in : p.d_out;
+        const uint32_t dst = ring + s * C::kStageBytes;
+        const bool in_width = col + c8 * 8 < width;
+        const int64_t shift = in_width ? col : -c8 * 8;   // (an address within the row in any case)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = r0 + 16 * i;
+          cp_async16(dst + r * 128 + ((c8 ^ (r & 7)) << 4), src[i] + shift, in_width && (have >> i & 1u));
+        }
+        const uint32_t wdst = dst + kRowsBytes;
+        const T* w = one ? u : v;
+        if (one == FWD) {
+          // rank rows of 64 columns, `width` apart
+          for (int j = r0; j < q.rank16; j += 16) {
+            const bool take = in_width && j < p.rank;
+            cp_async16(wdst + j * 128 + ((c8 ^ (j & 7)) << 4), w + (take ? j * width + col + c8 * 8 : 0), take);
+          }
+        } else {
+          // 64 rows of `rank` columns
+          const int j8 = t % (8 * RB);
+          if (j8 * 8 < q.rank16) {
+            for (int i = t / (8 * RB); i < kChunk; i += 16 / RB) {
+              const bool take = col + i < width && j8 * 8 < p.rank;
+              cp_async16(wdst + (j8 >> 3) * kBlockBytes + i * 128 + (((j8 & 7) ^ (i & 7)) << 4),
+                         w + (take ? (col + i) * p.rank + j8 * 8 : 0), take);
+            }
+          }
+        }
+        cp_async_commit();
+        if (it >= C::kLag) {
+          cp_async_wait<C::kLag>();
+          fence_async_shared();
+          mbar_arrive(full((it - C::kLag) % C::kStages));
+        }
+      }
+      cp_async_wait<0>();
+      if (ok) {
+        fence_async_shared();
+        for (int it = max(0, total - C::kLag); it < total; ++it) mbar_arrive(full(it % C::kStages));
+      }
+    } else if (warp == 8) {
+      // ---- tensor cores ----
+      bool ok = true;
+      for (int it = 0; it < n1; ++it) {
+        const int s = it % C::kStages;
+        if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x33))) break;
+        tc_fence_after_sync();
+        const uint32_t a = ring + s * C::kStageBytes, b = a + kRowsBytes;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint64_t ad = umma_smem_desc_sw128(a + kk * 32, 16, 1024);
+          const uint64_t bd = FWD ? umma_smem_desc_sw128(b + kk * 32, 16, 1024)
+                                  : umma_smem_desc_sw128(b + kk * 16 * 128, kBlockBytes, 1024);
+          umma_f16_elect(tmem, ad, bd, q.idesc1, it + kk > 0 ? 1u : 0u);
+        }
+        tc_commit_elect(free1(s));
+      }
+      if (ok && n1 > 0) tc_commit_elect(bar_sums);
+      if (ok && n2 > 0) ok = mbar_wait_long(wctx, bar_inner, 0, 0x34);
+      tc_fence_after_sync();
+      for (int j = 0; ok && j < n2; ++j) {
+        const int it = n1 + j, s = it % C::kStages, b = j & 1;
+        if (j >= 2 && !(ok = mbar_wait(wctx, out_free(b), ((j >> 1) - 1) & 1, 0x35))) break;
+        if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x36))) break;
+        tc_fence_after_sync();
+        const uint32_t w = ring + s * C::kStageBytes + kRowsBytes;
+        const uint32_t d = tmem + C::kOut + b * kChunk;
+        for (int kk = 0; kk < q.rank16 / 16; ++kk) {
+          const uint64_t bd = FWD ? umma_smem_desc_sw128(w + (kk >> 2) * kBlockBytes + (kk & 3) * 32, 16, 1024)
+                                  : umma_smem_desc_sw128(w + kk * 16 * 128, kBlockBytes, 1024);
+          umma_f16_tmem_a_elect(d, tmem + kk * 8, bd, q.idesc2, kk > 0 ? 1u : 0u);
+          umma_f16_tmem_a_elect(d, tmem + C::kLo + kk * 8, bd, q.idesc2, 1u);
+        }
+        tc_commit_elect(out_full(b));
+      }
+    } else if (warp < 4) {
+      // ---- epilogue: thread = row ----
+      const int r = threadIdx.x;
+      const int32_t row = row_of[r];
+      const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) << 21);
+      const float s = __ldg(p.scales + adapter);
+      const int blocks = q.rank16 / 16;
+      bool ok = n1 == 0 || mbar_wait_long(wctx, bar_sums, 0, 0x37);
+      float most = 0.f, down, up;
+      float* inner = p.inner != nullptr && rank == 0 && row >= 0 ? p.inner + static_cast<int64_t>(row) * p.rank : nullptr;
+      const float inner_scale = p.scale_inner ? s : 1.f;
+      if (ok) {
+        tc_fence_after_sync();
+        if (S > 1) {
+          // 16 bytes of rank 4j.. of row r at exchange + (j * 128 + r) * 16
+          for (int b = 0; b < blocks; ++b) {
+            uint32_t x[16];
+            if (n1 > 0) {
+              tmem_ld(lanes + b * 16, x);
+              tmem_wait_ld(x);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              st_shared_v4(exchange + ((b * 4 + i) * kTile + r) * 16, x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+          }
+          __syncwarp();
+          if (lane < S) mbar_arrive_cluster(bar_parts, lane);
+          ok = mbar_wait_cluster(wctx, bar_parts, 0, 0x38);
+        }
+      }
+      if (ok) {
+        for (int b = 0; b < blocks; ++b) {
+          uint32_t x[16];
+          if (S > 1) {
+            float sum[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+            for (int c = 0; c < S; ++c) {
+              const uint32_t from = cluster_map_shared(exchange, c);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float4 v = ld_shared_cluster_f4(from + ((b * 4 + i) * kTile + r) * 16);
+                sum[4 * i] += v.x;
+                sum[4 * i + 1] += v.y;
+                sum[4 * i + 2] += v.z;
+                sum[4 * i + 3] += v.w;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(sum[i]);
+            tmem_st16(lanes + b * 16, x);
+          } else {
+            tmem_ld(lanes + b * 16, x);
+            tmem_wait_ld(x);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(__uint_as_float(x[i])));
+          if (inner != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (b * 16 + i < p.rank) inner[b * 16 + i] = inner_scale * __uint_as_float(x[i]);
+          }
+        }
+        tmem_wait_st();
+        row_scale(most, &down, &up);
+        for (int b = 0; b < blocks; ++b) {
+          uint32_t x[16], hi[8], lo[8];
+          tmem_ld(lanes + b * 16, x);
+          tmem_wait_ld(x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float f0 = __uint_as_float(x[2 * i]) * down, f1 = __uint_as_float(x[2 * i + 1]) * down;
+            hi[i] = Pair<T>::pack(f0, f1);
+            const float2 h = Pair<T>::unpack(hi[i]);
+            lo[i] = Pair<T>::pack(f0 - h.x, f1 - h.y);
+          }
+          tmem_st8(lanes + b * 8, hi);
+          tmem_st8(lanes + C::kLo + b * 8, lo);
+        }
+        tmem_wait_st();
+        tc_fence_before_sync();
+        mbar_arrive(bar_inner);
+        const float c = s * up;
+        T* out = static_cast<T*>(p.out);
+        for (int j = 0; j < n2; ++j) {
+          const int it = n1 + j, st = it % C::kStages, b = j & 1;
+          if (!mbar_wait(wctx, out_full(b), (j >> 1) & 1, 0x39)) break;
+          if (!mbar_wait(wctx, full(st), (it / C::kStages) & 1, 0x3a)) break;
+          tc_fence_after_sync();
+          const uint32_t tile = ring + st * C::kStageBytes;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t d[32];
+            tmem_ld(lanes + C::kOut + b * kChunk + half * 32, d);
+            tmem_wait_ld(d);
+            if (half == 1) {
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(out_free(b));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t at = tile + r * 128 + (((half * 4 + i) ^ (r & 7)) << 4);
+              const uint4 y0 = ld_shared_v4(at);
+              uint32_t y[4] = {y0.x, y0.y, y0.z, y0.w};
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const float2 f = Pair<T>::unpack(y[w]);
+                y[w] = Pair<T>::pack(fmaf(c, __uint_as_float(d[i * 8 + w * 2]), f.x),
+                                     fmaf(c, __uint_as_float(d[i * 8 + w * 2 + 1]), f.y));
+              }
+              st_shared_v4(at, y[0], y[1], y[2], y[3]);
+            }
+          }
+          __syncwarp();
+          const int64_t col = static_cast<int64_t>(out0 + j) * kChunk + (lane & 7) * 8;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int rr = warp * 32 + i * 4 + (lane >> 3);
+            const uint4 y = ld_shared_v4(tile + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+            const int64_t dst_row = row_of[rr];
+            if (dst_row >= 0 && col < p.d_out) __stcs(reinterpret_cast<uint4*>(out + dst_row * p.ld_out + col), y);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(free2(st));
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  if (S > 1) cluster_sync();   // (nobody reads this CTA's partial sums any more)
+  else __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 8) tmem_dealloc(tmem, C::kTmemCols);
+}
+
+template <typename T, int RB, bool FWD>
+ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, cudaStream_t stream) {
+  using C = TileCfg<RB>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 0 && dev < 64 && !done[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(lora_tile_kernel<T, RB, FWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+      if (e != cudaSuccess) return cuda_status(e, where);
+      done[dev] = true;
+    }
+  }
+  launch_programmatic_cluster(lora_tile_kernel<T, RB, FWD>, static_cast<unsigned>(tiles * q.cluster), static_cast<unsigned>(q.cluster),
+                              true, kThreads, C::kSmem, stream, q);
+  KSB_CHECK_LAUNCH(where);
+  return KS_SUCCESS;
+}
+
+}  // namespace
+
+bool lora_tile_takes(const LoraPass& p) {
+  const auto rows16 = [](const void* m, int64_t ld) { return aligned16(m) && ld % 8 == 0; };
+  return p.rank % 8 == 0 && p.rank <= 128 && p.d_in % 8 == 0 && p.d_out % 8 == 0 && aligned16(p.u) && aligned16(p.v) &&
+         rows16(p.in, p.ld_in) && rows16(p.base, p.ld_base) && rows16(p.out, p.ld_out);
+}
+
+ks_status_t lora_tile_pass(const char* where, const LoraPass& p, bool forward, ks_dtype_t dtype, cudaStream_t stream) {
+  TileParams q = {};
+  q.p = p;
+  q.fault_word = kernel_fault_word();
+  q.rank16 = (p.rank + 15) / 16 * 16;
+  const uint32_t fmt = dtype == KS_DTYPE_F16 ? 0u : 1u;
+  q.idesc1 = umma_instr_desc(fmt, fmt, 0u, forward ? 0u : 1u, kTile, static_cast<uint32_t>(q.rank16));
+  q.idesc2 = umma_instr_desc(fmt, fmt, 0u, forward ? 0u : 1u, kTile, kChunk);
+  const int64_t tiles = lora_tile_bound(p.rows, p.adapters);
+  const bool wide = p.rank > 64;
+  const int64_t room = static_cast<int64_t>(sm_count()) * (wide ? 1 : 2);
+  const int64_t filled = (p.rows + kTile - 1) / kTile;
+  int s = 1;
+  while (s < kMaxCluster && filled * s * 2 <= room) s *= 2;
+  q.cluster = s;
+  if (tiles * s > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
+#define KSB_LORA_TILE(T)                                                                                                         \
+  (forward ? (wide ? launch_tile<T, 2, true>(where, q, tiles, stream) : launch_tile<T, 1, true>(where, q, tiles, stream))        \
+           : (wide ? launch_tile<T, 2, false>(where, q, tiles, stream) : launch_tile<T, 1, false>(where, q, tiles, stream)))
+  return dtype == KS_DTYPE_F16 ? KSB_LORA_TILE(__half) : KSB_LORA_TILE(__nv_bfloat16);
+#undef KSB_LORA_TILE
+}
+
+}  // namespace sm100
+}  // namespace ksb
