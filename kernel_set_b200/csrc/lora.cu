@@ -116,7 +116,11 @@ ks_status_t check_sizes(const char* where, int64_t rows, int adapters, int rank,
   return KS_SUCCESS;
 }
 
+// The workspace of the backward pass: g [rows, rank], then two maxima per row for f16 (LoraPass).
 int64_t inner_bytes(int64_t rows, int rank) { return (rows * rank * static_cast<int64_t>(sizeof(float)) + 255) / 256 * 256; }
+int64_t workspace_bytes_of(int64_t rows, int rank) {
+  return inner_bytes(rows, rank) + (2 * rows * static_cast<int64_t>(sizeof(float)) + 255) / 256 * 256;
+}
 
 }  // namespace
 }  // namespace ksb
@@ -181,7 +185,7 @@ ks_status_t ks_lora_backward_workspace(size_t* bytes, int64_t num_tokens, int nu
   KSB_REQUIRE_PTR(bytes);
   const ks_status_t st = check_sizes("ks_lora_backward_workspace", num_tokens, num_adapters, rank, k, n, KS_DTYPE_F16);
   if (st != KS_SUCCESS) return st;
-  *bytes = static_cast<size_t>(inner_bytes(num_tokens, rank));
+  *bytes = static_cast<size_t>(workspace_bytes_of(num_tokens, rank));
   return KS_SUCCESS;
 }
 
@@ -212,7 +216,7 @@ ks_status_t ks_lora_backward(void* d_x, int64_t ld_d_x, void* d_a, void* d_b, co
     KSB_FAIL(KS_ERROR_INVALID_ARGUMENT, "ks_lora_backward: in place, ld_d_x and ld_d_x_base must be equal");
   if (num_tokens > 0 && (d_x == d_out || d_x == x))
     KSB_FAIL(KS_ERROR_INVALID_ARGUMENT, "ks_lora_backward: d_x must be neither d_out nor x");
-  const size_t want = static_cast<size_t>(inner_bytes(num_tokens, rank));
+  const size_t want = static_cast<size_t>(workspace_bytes_of(num_tokens, rank));
   if (want > 0 && (workspace == nullptr || workspace_bytes < want || !aligned16(workspace)))
     KSB_FAIL(KS_ERROR_INVALID_ARGUMENT, "ks_lora_backward: workspace missing, too small or not 16-byte aligned");
   st = require_sm100(where);
@@ -221,21 +225,27 @@ ks_status_t ks_lora_backward(void* d_x, int64_t ld_d_x, void* d_a, void* d_b, co
   if (st != KS_SUCCESS) return st;
   cudaStream_t s = as_stream(stream);
   float* g = static_cast<float*>(workspace);
-  if (num_tokens > 0) {
-    LoraPass p = {};
-    p.out = d_x; p.base = d_x_base; p.in = d_out; p.u = b; p.v = a; p.scales = scales; p.ids = sorted_ids; p.offsets = offsets;
-    p.inner = g;
-    p.ld_out = ld_d_x; p.ld_base = ld_d_x_base; p.ld_in = ld_d_out;
-    p.rows = num_tokens; p.d_in = n; p.d_out = k;
-    p.u_j = 1; p.u_i = rank; p.v_o = 1; p.v_j = k;
-    p.adapters = num_adapters; p.rank = rank; p.scale_inner = true;
-    st = run_pass(where, p, false, dtype, s);
-    if (st != KS_SUCCESS) return st;
-  }
+  LoraPass p = {};
+  p.out = d_x; p.base = d_x_base; p.in = d_out; p.u = b; p.v = a; p.scales = scales; p.ids = sorted_ids; p.offsets = offsets;
+  p.inner = g;
+  p.ld_out = ld_d_x; p.ld_base = ld_d_x_base; p.ld_in = ld_d_out;
+  p.rows = num_tokens; p.d_in = n; p.d_out = k;
+  p.u_j = 1; p.u_i = rank; p.v_o = 1; p.v_j = k;
+  p.adapters = num_adapters; p.rank = rank; p.scale_inner = true;
   LoraWeightGrad w = {};
   w.d_a = d_a; w.d_b = d_b; w.x = x; w.d_out = d_out; w.g = g; w.h = h; w.scales = scales; w.ids = sorted_ids; w.offsets = offsets;
   w.ld_x = ld_x; w.ld_d_out = ld_d_out; w.rows = num_tokens; w.k = k; w.n = n; w.adapters = num_adapters; w.rank = rank;
-  return run_weight_grad(where, w, dtype, s);
+  const bool tensor = sm100::lora_tile_takes(p) && sm100::lora_weight_grad_takes(w);
+  if (tensor && dtype == KS_DTYPE_F16 && num_tokens > 0) {
+    p.h = h;
+    w.most_g = p.most_g = reinterpret_cast<float*>(static_cast<char*>(workspace) + inner_bytes(num_tokens, rank));
+    w.most_h = p.most_h = p.most_g + num_tokens;
+  }
+  if (num_tokens > 0) {
+    st = run_pass(where, p, false, dtype, s);
+    if (st != KS_SUCCESS) return st;
+  }
+  return tensor ? sm100::lora_weight_grad_pass(where, w, dtype, s) : run_weight_grad(where, w, dtype, s);
 }
 
 }  // extern "C"

@@ -135,6 +135,13 @@ __device__ __forceinline__ void row_scale(float most, float* down, float* up) {
   *up = __uint_as_float(e << 23);
 }
 
+// The largest of the warp's values.
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
 struct TileParams {
   LoraPass p;
   unsigned int* fault_word;
@@ -247,6 +254,7 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
     if (lane == 0) {
       words[2] = static_cast<uint32_t>(f.adapter);
       words[3] = static_cast<uint32_t>(f.count);
+      words[4] = static_cast<uint32_t>(f.place);
     }
     for (int i = lane; i < kTile; i += 32) row_of[i] = i < f.count ? static_cast<int32_t>(lora_row(p.ids, f.place + i, p.rows)) : -1;
   }
@@ -257,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
   const uint32_t tmem = words[0];
   const int adapter = static_cast<int>(words[2]);
   const int count = static_cast<int>(words[3]);
+  const int64_t place = words[4];
 
   // this CTA's 64-column chunks of the inputs and of the outputs
   const int in_chunks = static_cast<int>((p.d_in + kChunk - 1) / kChunk), out_chunks = static_cast<int>((p.d_out + kChunk - 1) / kChunk);
@@ -455,6 +464,21 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
         }
         tmem_wait_st();
         row_scale(most, &down, &up);
+        if (p.most_g != nullptr && rank == 0) {
+          float most_h = 0.f;
+          if (row >= 0)
+            for (int i = 0; i < p.rank; i += 4) {
+              const float4 v = __ldg(reinterpret_cast<const float4*>(p.h + static_cast<int64_t>(row) * p.rank + i));
+              most_h = fmaxf(fmaxf(fmaxf(most_h, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+            }
+          most_h = warp_max(most_h);
+          const float most_g = warp_max(row >= 0 ? most * fabsf(inner_scale) : 0.f);
+          if (lane == 0 && warp * 32 < count) {
+            const int64_t at = place + warp * 32;
+            p.most_g[at] = most_g;
+            p.most_h[at] = most_h;
+          }
+        }
         for (int b = 0; b < blocks; ++b) {
           uint32_t x[16], hi[8], lo[8];
           tmem_ld(lanes + b * 16, x);
@@ -548,6 +572,309 @@ ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, c
   return KS_SUCCESS;
 }
 
+// ---------------------------------------------------------------------------------
+// gradients of the factors
+// ---------------------------------------------------------------------------------
+// dA^T [k, rank] = sum over the adapter's rows of x_row g_row^T, and dB [n, rank] = s sum dout_row h_row^T: the same product of a
+// matrix of 16-bit rows, taken in slabs of 256 columns, with fp32 vectors of `rank` numbers. A cluster of CTAs has a slab of one
+// adapter and splits its rows; the parts are added up over distributed shared memory in rank order. Rows are contracted, so both operands
+// are stored with the contracted index outside (MN-major), as they lie in memory; a vector is split into two 16-bit
+// numbers, two MMAs. In f16 the vectors are scaled by a power of two per adapter, from the maxima that the pass before left.
+//   warps 0-3   split vectors (registers, a stage ahead -> shared memory), at the end the sums and the result
+//   warps 4-7   copies of 64 rows x 512 bytes by cp.async
+//   warp 8      tcgen05.mma: per stage 2 (128-column halves) x 4 (16 rows each) x 2 (parts), N = rank
+// Bound by memory: every element of x and dout is read once; the vectors are read again from L2 per slab (half the bytes of
+// a slab's rows at rank 64, which is why a slab is as wide as tensor memory and the ring allow two CTAs per SM).
+constexpr int kSlab = 256;
+
+template <int RB>
+struct GradCfg {
+  static constexpr int kStages = RB == 1 ? 2 : 3;
+  static constexpr int kLag = kStages - 1;
+  static constexpr int kRows = 64 * kSlab * 2;             // four blocks of 64 rows x 128 bytes
+  static constexpr int kPart = RB * kBlockBytes;           // one 16-bit part of the vectors
+  static constexpr int kStageBytes = kRows + 2 * kPart;
+  static constexpr int kTmemCols = RB == 1 ? 128 : 256;    // two sums of 64 RB columns
+  static constexpr int kPerSm = RB == 1 ? 2 : 1;
+  static constexpr int kBars = 2 * kStages + 1;
+  static constexpr int kSums = kSlab * 64 * RB * 4;        // over the ring, once it is drained
+  static_assert(kSums <= kStages * kStageBytes, "the sums lie over the ring");
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + 8 * kBars + 64;
+  static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory");
+};
+
+struct GradParams {
+  LoraWeightGrad p;
+  unsigned int* fault_word;
+  uint32_t idesc;
+  int rank16, cluster;
+  int slabs_a, slabs;     // slabs of x, of both
+};
+
+template <typename T, int RB>
+__global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_grad_kernel(const __grid_constant__ GradParams q) {
+  using C = GradCfg<RB>;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const LoraWeightGrad& p = q.p;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t ring = smem_u32(smem);
+  uint64_t* bar_mem = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes);
+  const uint32_t bars = smem_u32(bar_mem);
+  const auto full = [&](int s) { return bars + 8u * s; };
+  const auto freed = [&](int s) { return bars + 8u * (C::kStages + s); };
+  const uint32_t bar_sums = bars + 8u * (2 * C::kStages);
+  volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(bar_mem + C::kBars);
+  const WaitCtx wctx{smem_u32(const_cast<uint32_t*>(words) + 1), q.fault_word};
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int S = q.cluster;
+  const int rank = blockIdx.x % S;
+  const int item = blockIdx.x / S;
+  const int adapter = item / q.slabs;
+  const int slab = item - adapter * q.slabs;
+  const bool is_a = slab < q.slabs_a;
+  const int64_t col0 = static_cast<int64_t>(is_a ? slab : slab - q.slabs_a) * kSlab;
+  const int64_t width = is_a ? p.k : p.n;
+  const T* rows = static_cast<const T*>(is_a ? p.x : p.d_out);
+  const int64_t ld = is_a ? p.ld_x : p.ld_d_out;
+  const float* vecs = is_a ? p.g : p.h;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(full(s), 2 * kProdThreads);
+      mbar_init(freed(s), 1);
+    }
+    mbar_init(bar_sums, 1);
+    words[1] = 0u;
+    fence_barrier_init();
+  }
+  grid_dependency_wait();
+  if (warp == 8) {   // (behind the wait: a kernel that still runs may need the columns)
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(words)), C::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = words[0];
+  const int64_t begin = lora_offset(p.offsets, adapter, p.rows);
+  const int64_t count = max(lora_offset(p.offsets, adapter + 1, p.rows) - begin, int64_t(0));
+  const int64_t chunks = (count + 63) / 64;
+  const int64_t chunk0 = chunks * rank / S;
+  const int n = static_cast<int>(chunks * (rank + 1) / S - chunk0);
+  const auto row_at = [&](int64_t chunk, int i) -> int32_t {   // row i of a chunk, -1 past the end
+    const int64_t at = chunk * 64 + i;
+    return at < count ? static_cast<int32_t>(lora_row(p.ids, begin + at, p.rows)) : -1;
+  };
+  float up = 1.f;
+
+  if (warp >= 4 && warp < 8) {
+    // ---- copies: a warp takes every fourth row, a lane 16 bytes of it ----
+    const int w = warp - 4;
+    const int64_t col = col0 + lane * 8;
+    const bool in_width = col < width;
+    const T* src = rows + (in_width ? col : 0);
+    const uint32_t dst0 = ring + (lane >> 3) * kBlockBytes;
+    bool ok = true;
+    int32_t mine = n > 0 ? row_at(chunk0, w + 4 * (lane & 15)) : -1;   // lane i < 16: row w + 4 i
+#pragma unroll 1
+    for (int it = 0; it < n; ++it) {
+      const int s = it % C::kStages;
+      if (it >= C::kStages && !(ok = mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x41))) break;
+      const int32_t now = mine;
+      if (it + 1 < n) mine = row_at(chunk0 + it + 1, w + 4 * (lane & 15));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int32_t row = __shfl_sync(0xffffffffu, now, i);
+        const int r = w + 4 * i;
+        cp_async16(dst0 + s * C::kStageBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4), src + (row >= 0 ? row : 0) * ld,
+                   in_width && row >= 0);
+      }
+      cp_async_commit();
+      if (it >= C::kLag) {
+        cp_async_wait<C::kLag>();
+        fence_async_shared();
+        mbar_arrive(full((it - C::kLag) % C::kStages));
+      }
+    }
+    cp_async_wait<0>();
+    if (ok) {
+      fence_async_shared();
+      for (int it = max(0, n - C::kLag); it < n; ++it) mbar_arrive(full(it % C::kStages));
+    }
+  } else if (warp < 4) {
+    // ---- vectors: a thread takes 8 ranks of every (16 / RB)-th row ----
+    const int t = threadIdx.x;
+    const int c8 = t % (8 * RB), r0 = t / (8 * RB);
+    constexpr int kStep = 16 / RB, kMine = 64 / kStep;
+    const bool used = c8 * 8 < q.rank16, has = c8 * 8 < p.rank;
+    float down = 1.f;
+    if (std::is_same<T, __half>::value) {
+      const float* most = is_a ? p.most_g : p.most_h;
+      float m = 0.f;
+      for (int64_t i = lane; i * 32 < count; i += 32) m = fmaxf(m, __ldg(most + begin + i * 32));
+      row_scale(warp_max(m), &down, &up);
+    }
+    int32_t row[kMine];
+    float4 v[kMine][2];
+    const auto find = [&](int64_t chunk) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) row[i] = used ? row_at(chunk, r0 + i * kStep) : -1;
+    };
+    const auto load = [&] {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const bool take = has && row[i] >= 0;
+        const float4* from = reinterpret_cast<const float4*>(vecs + static_cast<int64_t>(take ? row[i] : 0) * p.rank + (take ? c8 * 8 : 0));
+        v[i][0] = take ? __ldg(from) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[i][1] = take ? __ldg(from + 1) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    };
+    bool ok = true;
+    if (n > 0) {
+      find(chunk0);
+      load();
+      if (n > 1) find(chunk0 + 1);
+    }
+#pragma unroll 1
+    for (int it = 0; it < n; ++it) {
+      const int s = it % C::kStages;
+      if (it >= C::kStages && !(ok = mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x42))) break;
+      const uint32_t dst = ring + s * C::kStageBytes + C::kRows + (c8 >> 3) * kBlockBytes;
+      if (used) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int r = r0 + i * kStep;
+          const float f[8] = {v[i][0].x * down, v[i][0].y * down, v[i][0].z * down, v[i][0].w * down,
+                              v[i][1].x * down, v[i][1].y * down, v[i][1].z * down, v[i][1].w * down};
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            hi[j] = Pair<T>::pack(f[2 * j], f[2 * j + 1]);
+            const float2 h = Pair<T>::unpack(hi[j]);
+            lo[j] = Pair<T>::pack(f[2 * j] - h.x, f[2 * j + 1] - h.y);
+          }
+          const uint32_t at = dst + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
+          st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
+          st_shared_v4(at + C::kPart, lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      fence_async_shared();
+      mbar_arrive(full(s));
+      if (it + 1 < n) load();
+      if (it + 2 < n) find(chunk0 + it + 2);
+    }
+  } else if (n > 0) {
+    // ---- tensor cores ----
+    bool ok = true;
+    for (int it = 0; it < n; ++it) {
+      const int s = it % C::kStages;
+      if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x43))) break;
+      tc_fence_after_sync();
+      const uint32_t a = ring + s * C::kStageBytes, b = a + C::kRows;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const uint64_t ad = umma_smem_desc_sw128(a + half * 2 * kBlockBytes + kk * 2048, kBlockBytes, 1024);
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+            umma_f16_elect(tmem + half * 64 * RB, ad, umma_smem_desc_sw128(b + part * C::kPart + kk * 2048, kBlockBytes, 1024), q.idesc,
+                           it + kk + part > 0 ? 1u : 0u);
+        }
+      }
+      tc_commit_elect(freed(s));
+    }
+    if (ok) tc_commit_elect(bar_sums);
+  }
+
+  // sums [rank][256 columns] fp32 over the ring
+  if (warp < 4) {
+    const int blocks = q.rank16 / 16;
+    const bool have = n > 0 && mbar_wait_long(wctx, bar_sums, 0, 0x44);
+    tc_fence_after_sync();
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) << 21);
+    const float c = is_a ? up : up * __ldg(p.scales + adapter);
+    for (int half = 0; half < 2; ++half)
+      for (int b = 0; b < blocks; ++b) {
+        uint32_t x[16];
+        if (have) {
+          tmem_ld(lanes + half * 64 * RB + b * 16, x);
+          tmem_wait_ld(x);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          st_shared_f32(ring + ((b * 16 + i) * kSlab + half * 128 + threadIdx.x) * 4, have ? c * __uint_as_float(x[i]) : 0.f);
+      }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  if (S > 1) cluster_sync();
+  else __syncthreads();
+  // the cluster's CTAs share the slab's columns; 8 numbers that lie together in the result at a time
+  const int cols = kSlab / S;   // a multiple of 8
+  const int64_t factor = static_cast<int64_t>(adapter) * p.rank * width;
+  const auto sum_at = [&](int j, int m, int cta) {
+    return cluster_map_shared(ring + (j * kSlab + m) * 4, cta);
+  };
+  if (is_a) {
+    T* out = static_cast<T*>(p.d_a) + factor;
+    for (int e = threadIdx.x; e < p.rank * (cols / 8); e += kThreads) {
+      const int j = e / (cols / 8), m = rank * cols + (e % (cols / 8)) * 8;
+      if (col0 + m >= width) continue;
+      float f[8] = {};
+      for (int cta = 0; cta < S; ++cta) {
+        const float4 a = ld_shared_cluster_f4(sum_at(j, m, cta)), b = ld_shared_cluster_f4(sum_at(j, m + 4, cta));
+        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
+        f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+      }
+      *reinterpret_cast<uint4*>(out + j * width + col0 + m) =
+          make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]), Pair<T>::pack(f[6], f[7]));
+    }
+  } else {
+    T* out = static_cast<T*>(p.d_b) + factor;
+    for (int e = threadIdx.x; e < p.rank / 8 * cols; e += kThreads) {
+      const int j = e / cols * 8, m = rank * cols + e % cols;
+      if (col0 + m >= width) continue;
+      float f[8] = {};
+      for (int cta = 0; cta < S; ++cta)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float v;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sum_at(j + i, m, cta)) : "memory");
+          f[i] += v;
+        }
+      *reinterpret_cast<uint4*>(out + (col0 + m) * p.rank + j) =
+          make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]), Pair<T>::pack(f[6], f[7]));
+    }
+  }
+  __syncwarp();
+  if (S > 1) cluster_sync();   // (nobody reads this CTA's sums any more)
+  else __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 8) tmem_dealloc(tmem, C::kTmemCols);
+}
+
+template <typename T, int RB>
+ks_status_t launch_grad(const char* where, const GradParams& q, int64_t items, cudaStream_t stream) {
+  using C = GradCfg<RB>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 0 && dev < 64 && !done[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(lora_weight_grad_kernel<T, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+      if (e != cudaSuccess) return cuda_status(e, where);
+      done[dev] = true;
+    }
+  }
+  launch_programmatic_cluster(lora_weight_grad_kernel<T, RB>, static_cast<unsigned>(items * q.cluster), static_cast<unsigned>(q.cluster),
+                              true, kThreads, C::kSmem, stream, q);
+  KSB_CHECK_LAUNCH(where);
+  return KS_SUCCESS;
+}
+
 }  // namespace
 
 bool lora_tile_takes(const LoraPass& p) {
@@ -577,6 +904,32 @@ ks_status_t lora_tile_pass(const char* where, const LoraPass& p, bool forward, k
            : (wide ? launch_tile<T, 2, false>(where, q, tiles, stream) : launch_tile<T, 1, false>(where, q, tiles, stream)))
   return dtype == KS_DTYPE_F16 ? KSB_LORA_TILE(__half) : KSB_LORA_TILE(__nv_bfloat16);
 #undef KSB_LORA_TILE
+}
+
+bool lora_weight_grad_takes(const LoraWeightGrad& p) {
+  return p.rank % 8 == 0 && p.rank <= 128 && p.k % 8 == 0 && p.n % 8 == 0 && p.ld_x % 8 == 0 && p.ld_d_out % 8 == 0 && aligned16(p.x) &&
+         aligned16(p.d_out) && aligned16(p.d_a) && aligned16(p.d_b) && aligned16(p.g) && aligned16(p.h);
+}
+
+ks_status_t lora_weight_grad_pass(const char* where, const LoraWeightGrad& p, ks_dtype_t dtype, cudaStream_t stream) {
+  GradParams q = {};
+  q.p = p;
+  q.fault_word = kernel_fault_word();
+  q.rank16 = (p.rank + 15) / 16 * 16;
+  const uint32_t fmt = dtype == KS_DTYPE_F16 ? 0u : 1u;
+  q.idesc = umma_instr_desc(fmt, fmt, 1u, 1u, 128u, static_cast<uint32_t>(q.rank16));
+  q.slabs_a = static_cast<int>((p.k + kSlab - 1) / kSlab);
+  q.slabs = q.slabs_a + static_cast<int>((p.n + kSlab - 1) / kSlab);
+  const bool wide = p.rank > 64;
+  const int64_t items = static_cast<int64_t>(p.adapters) * q.slabs;
+  const int64_t room = static_cast<int64_t>(sm_count()) * (wide ? 1 : 2);
+  int s = 1;
+  while (s < kMaxCluster && items * s * 2 <= room && p.rows > 64 * s) s *= 2;
+  q.cluster = s;
+  if (items * s > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
+  if (dtype == KS_DTYPE_F16)
+    return wide ? launch_grad<__half, 2>(where, q, items, stream) : launch_grad<__half, 1>(where, q, items, stream);
+  return wide ? launch_grad<__nv_bfloat16, 2>(where, q, items, stream) : launch_grad<__nv_bfloat16, 1>(where, q, items, stream);
 }
 
 }  // namespace sm100

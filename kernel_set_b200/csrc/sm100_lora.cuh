@@ -22,5 +22,9 @@ bool lora_tile_takes(const LoraPass& p);
 // forward: U [rank, d_in], V [d_out, rank] as stored; otherwise U and V are the transposes of what is stored.
 ks_status_t lora_tile_pass(const char* where, const LoraPass& p, bool forward, ks_dtype_t dtype, cudaStream_t stream);
 
+// The factors' gradients, where lora_tile_takes the pass before them and the gradients and x are 16-byte aligned.
+bool lora_weight_grad_takes(const LoraWeightGrad& p);
+ks_status_t lora_weight_grad_pass(const char* where, const LoraWeightGrad& p, ks_dtype_t dtype, cudaStream_t stream);
+
 }  // namespace sm100
 }  // namespace ksb

@@ -210,6 +210,8 @@ def test_inner_vector_beyond_f16(ks, cuda, tokens, dtype, size):
     out = ks.lora.apply(torch.empty_like(p.base), p.base, p.x, p.a, p.b, p.scales, ids, offsets)
     check("out", out, want, bound + tiny)
     p.scales = p.scales * size ** 2
+    if size > 1:   # (so that the factors' gradients fit)
+        p.d_out = (p.d_out.float() * 2.0 ** -9).to(dtype)
     hf = h.float()
     want, bounds = p.backward(hf)
     fits = [w.abs().max() < torch.finfo(dtype).max for w in want]
