@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kMaxAnyRank = 4096;
 constexpr int kAnyThreads = 256;
+constexpr int kFewRows = 256;   // up to which the forward pass takes 8 rows at a time
 
 // Any rank, widths and alignment: a CTA per place. The warps take the ranks in turn, a lane every 32nd product of a
 // sum; then a thread takes every 256th output.
@@ -86,7 +87,10 @@ __global__ void __launch_bounds__(kAnyThreads) lora_weight_grad_any_kernel(LoraW
 }
 
 ks_status_t run_pass(const char* where, const LoraPass& p, bool forward, ks_dtype_t dtype, cudaStream_t s) {
-  if (sm100::lora_tile_takes(p)) return sm100::lora_tile_pass(where, p, forward, dtype, s);
+  if (sm100::lora_tile_takes(p)) {
+    if (forward && p.rows <= kFewRows) return sm100::lora_few_pass(where, p, dtype, s);
+    return sm100::lora_tile_pass(where, p, forward, dtype, s);
+  }
   const unsigned grid = static_cast<unsigned>(p.rows);
   const size_t smem = static_cast<size_t>(p.rank) * sizeof(float);
   if (dtype == KS_DTYPE_F16) sm100::launch_programmatic(lora_any_kernel<__half>, grid, kAnyThreads, smem, s, p);

@@ -1,0 +1,96 @@
+// Device code shared by the adapters' tensor-core kernels: 16-bit pairs, the scale of an inner vector, and where a tile lies.
+#pragma once
+
+#include "common.cuh"
+#include "lora_math.cuh"
+
+namespace ksb {
+namespace sm100 {
+
+template <typename T>
+struct Pair;   // two 16-bit numbers in a word
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+};
+
+// The power of two 2^-e for a row whose largest magnitude is `most`, so that most 2^-e is in [1, 2) where possible, and 2^e.
+// It keeps what f16 could not hold (sums beyond 65504, small ones whose low part would vanish) exact; 1 for zeros and non-finite rows.
+__device__ __forceinline__ void row_scale(float most, float* down, float* up) {
+  uint32_t e = (__float_as_uint(most) >> 23) & 255u;
+  if (e == 0u || e == 255u) e = 127u;
+  e = e > 253u ? 253u : e;
+  *down = __uint_as_float((254u - e) << 23);
+  *up = __uint_as_float(e << 23);
+}
+
+// Where tile `index` lies: adapter (`adapters` for the rows without one, -1 past the last tile), first place and row count.
+struct TilePlace {
+  int adapter;
+  int count;
+  int64_t place;
+};
+
+// Found by one warp: a lane counts the tiles of a run of adapters, the one whose run holds the tile walks it again.
+template <int TILE>
+__device__ __forceinline__ TilePlace find_tile(const int32_t* __restrict__ offsets, int adapters, int64_t rows, int64_t index) {
+  const int lane = threadIdx.x & 31;
+  const int groups = adapters + 1;
+  const int run = (groups + 31) / 32;
+  const int first = lane * run < groups ? lane * run : groups;
+  const int last = first + run < groups ? first + run : groups;
+  const auto begin_of = [&](int g) { return g > adapters ? rows : lora_offset(offsets, g, rows); };
+  int64_t mine = 0;
+#pragma unroll 4
+  for (int g = first; g < last; ++g) {
+    const int64_t n = begin_of(g + 1) - begin_of(g);
+    mine += n > 0 ? (n + TILE - 1) / TILE : 0;
+  }
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  TilePlace f{-1, 0, 0};
+  const bool here = index < upto && index >= upto - mine;
+  if (here) {
+    int64_t left = index - (upto - mine);
+    for (int g = first; g < last; ++g) {
+      const int64_t b = begin_of(g), n = begin_of(g + 1) - b;
+      const int64_t tiles = n > 0 ? (n + TILE - 1) / TILE : 0;
+      if (left < tiles) {
+        f.adapter = g;
+        f.place = b + left * TILE;
+        const int64_t rest = n - left * TILE;
+        f.count = static_cast<int>(rest < TILE ? rest : TILE);
+        break;
+      }
+      left -= tiles;
+    }
+  }
+  const unsigned who = __ballot_sync(0xffffffffu, here);
+  if (who == 0u) return f;
+  const int src = __ffs(who) - 1;
+  f.adapter = __shfl_sync(0xffffffffu, f.adapter, src);
+  f.count = __shfl_sync(0xffffffffu, f.count, src);
+  f.place = __shfl_sync(0xffffffffu, f.place, src);
+  return f;
+}
+
+}  // namespace sm100
+}  // namespace ksb
