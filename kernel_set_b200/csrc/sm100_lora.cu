@@ -3,7 +3,7 @@
 //
 // A tile is up to 128 rows of one adapter, and one cluster of CTAs does both products of it: each CTA multiplies its slice
 // of U's columns with the rows' elements there, the partial sums [128 x rank] are added up over distributed shared memory
-// (every CTA adds all of them, in rank order, so all hold the same bits), and each CTA gives its slice of the outputs. The
+// (in rank order, so all CTAs hold the same bits), and each CTA gives its slice of the outputs. The
 // inner vectors never leave the SM, there is one launch, and while the partial sums are exchanged the rows of y0 and V's
 // tiles are already on their way: both phases draw on one ring of shared-memory stages.
 //   warps 0-3   epilogue: a thread per row. Partial sums out of tensor memory, exchange, split into two 16-bit numbers,
@@ -31,16 +31,15 @@ constexpr int kTile = kLoraTile;
 constexpr int kChunk = 64;                         // columns of a stage: 128 bytes
 constexpr int kRowsBytes = kTile * kChunk * 2;     // rows' part of a stage
 constexpr int kBlockBytes = 64 * kChunk * 2;       // 64 rows x 128 bytes of a factor
-constexpr int kEpiWarps = 4, kProdWarps = 4;
+constexpr int kEpiWarps = 4, kProdWarps = 4, kMmaWarp = kEpiWarps + kProdWarps;
 constexpr int kProdThreads = kProdWarps * 32;
-constexpr int kThreads = (kEpiWarps + kProdWarps + 1) * 32;
+constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kMaxCluster = 8;
 
 // RB: 64-rank blocks (rank <= 64 RB).
 template <int RB>
 struct TileCfg {
   static constexpr int kStages = RB == 1 ? 3 : 4;
-  static constexpr int kLag = kStages - 1;          // stages whose copies are in flight behind the one being issued
   static constexpr int kStageBytes = kRowsBytes + RB * kBlockBytes;
   static constexpr int kExchange = kTile * 64 * RB * 4;
   static constexpr int kLo = 64 * RB;               // tensor memory: sums / high part, low part, two output buffers
@@ -48,7 +47,7 @@ struct TileCfg {
   static constexpr int kTmemCols = RB == 1 ? 256 : 512;
   static constexpr int kPerSm = RB == 1 ? 2 : 1;
   static_assert(kOut + 2 * kChunk <= kTmemCols, "tensor memory layout");
-  static constexpr int kBars = 3 * kStages + 7;
+  static constexpr int kBars = 3 * kStages + 8;
   static constexpr int kSmem = 1024 + kStages * kStageBytes + kExchange + kTile * 4 + 8 * kBars + 64;
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory");
 };
@@ -56,11 +55,16 @@ struct TileCfg {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// What this thread's copies (or stores) wrote to shared memory, for the tensor cores to read.
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// What copies and stores wrote to shared memory before this point, for the tensor cores to read behind it.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Arrives on the barrier once all copies that this thread has issued are complete. (The barrier counts the arrival; the thread
+// that lets the tensor cores read the stage runs fence_async_shared() behind its wait. A producer that waits for its copies
+// itself, to place the fence, holds up the next stage's: 113 us against 84 for 16384 rows beside 4096 x 4096, rank 64.)
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 
 // Arrives on the barrier at the same place in the cluster's CTA `rank`; orders this thread's earlier writes.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, uint32_t rank) {
@@ -89,6 +93,9 @@ __device__ __forceinline__ bool mbar_wait_cluster(const WaitCtx& ctx, uint32_t b
       return false;
     }
   }
+}
+__device__ __forceinline__ void st_shared_cluster_f4(uint32_t addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 // Lane i of the warp writes 8 consecutive columns of tensor memory lane (taddr.lane + i).
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -137,8 +144,9 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
   const uint32_t bar_sums = bars + 8u * (3 * C::kStages);        // first product complete
   const uint32_t bar_inner = bar_sums + 8;                       // second product's operand is in tensor memory
   const uint32_t bar_parts = bar_sums + 16;                      // the cluster's partial sums are in shared memory
-  const auto out_full = [&](int b) { return bar_sums + 24u + 8u * b; };
-  const auto out_free = [&](int b) { return bar_sums + 40u + 8u * b; };
+  const uint32_t bar_total = bar_sums + 24;                      // and so are their totals
+  const auto out_full = [&](int b) { return bar_sums + 32u + 8u * b; };
+  const auto out_free = [&](int b) { return bar_sums + 48u + 8u * b; };
   volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(bar_mem + C::kBars);   // tmem address, abort, tile
   const WaitCtx wctx{smem_u32(const_cast<uint32_t*>(words) + 1), q.fault_word};
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -154,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
     mbar_init(bar_sums, 1);
     mbar_init(bar_inner, kEpiWarps * 32);
     mbar_init(bar_parts, static_cast<uint32_t>(S) * kEpiWarps);
+    mbar_init(bar_total, static_cast<uint32_t>(S) * kEpiWarps);
     for (int b = 0; b < 2; ++b) {
       mbar_init(out_full(b), 1);
       mbar_init(out_free(b), kEpiWarps);
@@ -162,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
     fence_barrier_init();
   }
   grid_dependency_wait();
-  if (warp == 8) {   // (behind the wait: a kernel that still runs may need the columns)
+  if (warp == kMmaWarp) {   // (behind the wait: a kernel that still runs may need the columns)
     tmem_alloc(smem_u32(const_cast<uint32_t*>(words)), C::kTmemCols);
     tmem_relinquish();
   }
@@ -207,83 +216,79 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
     }
   } else if (adapter >= 0) {
     const int total = n1 + n2;
-    if (warp >= 4 && warp < 8) {
+    if (warp >= kEpiWarps && warp < kMmaWarp) {
       // ---- producer ----
       const int t = threadIdx.x - kEpiWarps * 32;
-      const int c8 = t & 7, r0 = t >> 3;
+      const int c8 = t & 7, r0 = t >> 3;                         // rows' part: 16 bytes of the rows r0 + 16 i
+      const int j8 = t % (8 * RB), i0 = t / (8 * RB);            // 64 rows of `rank` columns: rows i0 + 16 / RB * i
       const T* u = static_cast<const T*>(p.u) + static_cast<int64_t>(adapter) * p.rank * p.d_in;
       const T* v = static_cast<const T*>(p.v) + static_cast<int64_t>(adapter) * p.rank * p.d_out;
       const T* src[8];
       uint32_t have = 0u;
-      const auto aim = [&](const void* m, int64_t ld) {
+      const auto aim = [&](const void* m, int64_t ld, int chunk) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int32_t row = row_of[r0 + 16 * i];
           if (row >= 0) have |= 1u << i;
-          src[i] = static_cast<const T*>(m) + (row >= 0 ? row : 0) * ld + c8 * 8;
+          src[i] = static_cast<const T*>(m) + (row >= 0 ? row : 0) * ld + static_cast<int64_t>(chunk) * kChunk + c8 * 8;
         }
       };
-      aim(p.in, p.ld_in);
-      bool ok = true;
-      const int first2 = n1 % C::kStages;   // stage of the second phase's first chunk
+      aim(p.in, p.ld_in, in0);
 #pragma unroll 1
       for (int it = 0; it < total; ++it) {
         const int s = it % C::kStages;
         const int before = it - C::kStages;   // the stage's last use
         if (before >= 0) {
-          if (before < n1) ok = mbar_wait(wctx, free1(s), (before / C::kStages) & 1, 0x31);
-          else ok = mbar_wait(wctx, free2(s), ((before - n1 - (s - first2 + C::kStages) % C::kStages) / C::kStages) & 1, 0x32);
-          if (!ok) break;
+          const int n2_before = before - n1;
+          const uint32_t bar = n2_before < 0 ? free1(s) : free2(s);
+          const uint32_t parity = (n2_before < 0 ? before / C::kStages : n2_before / C::kStages) & 1;
+          if (!mbar_wait(wctx, bar, parity, 0x31)) break;
         }
-        if (it == n1) aim(p.base, p.ld_base);
+        if (it == n1) aim(p.base, p.ld_base, out0);
         const bool one = it < n1;
         const int64_t col = static_cast<int64_t>(one ? in0 + it : out0 + it - n1) * kChunk;
         const int64_t width = one ? p.d_in : p.d_out;
         const uint32_t dst = ring + s * C::kStageBytes;
         const bool in_width = col + c8 * 8 < width;
-        const int64_t shift = in_width ? col : -c8 * 8;   // (an address within the row in any case)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int r = r0 + 16 * i;
-          cp_async16(dst + r * 128 + ((c8 ^ (r & 7)) << 4), src[i] + shift, in_width && (have >> i & 1u));
+          const bool take = in_width && (have >> i & 1u);
+          cp_async16(dst + r0 * 128 + ((c8 ^ (r0 & 7)) << 4) + i * 2048, take ? src[i] : p.in, take);
+          src[i] += kChunk;
         }
         const uint32_t wdst = dst + kRowsBytes;
         const T* w = one ? u : v;
         if (one == FWD) {
           // rank rows of 64 columns, `width` apart
-          for (int j = r0; j < q.rank16; j += 16) {
+          const T* from = w + r0 * width + col + c8 * 8;
+#pragma unroll
+          for (int i = 0; i < 4 * RB; ++i) {
+            const int j = r0 + 16 * i;
             const bool take = in_width && j < p.rank;
-            cp_async16(wdst + j * 128 + ((c8 ^ (j & 7)) << 4), w + (take ? j * width + col + c8 * 8 : 0), take);
+            if (i * 16 < q.rank16)
+              cp_async16(wdst + r0 * 128 + ((c8 ^ (r0 & 7)) << 4) + i * 2048, take ? from + i * 16 * width : p.u, take);
           }
-        } else {
+        } else if (j8 * 8 < q.rank16) {
           // 64 rows of `rank` columns
-          const int j8 = t % (8 * RB);
-          if (j8 * 8 < q.rank16) {
-            for (int i = t / (8 * RB); i < kChunk; i += 16 / RB) {
-              const bool take = col + i < width && j8 * 8 < p.rank;
-              cp_async16(wdst + (j8 >> 3) * kBlockBytes + i * 128 + (((j8 & 7) ^ (i & 7)) << 4),
-                         w + (take ? (col + i) * p.rank + j8 * 8 : 0), take);
-            }
+          const T* from = w + (col + i0) * p.rank + j8 * 8;
+#pragma unroll
+          for (int i = 0; i < 4 * RB; ++i) {
+            const int r = i0 + 16 / RB * i;
+            const bool take = col + r < width && j8 * 8 < p.rank;
+            cp_async16(wdst + (j8 >> 3) * kBlockBytes + r * 128 + (((j8 & 7) ^ (r & 7)) << 4),
+                       take ? from + static_cast<int64_t>(16 / RB * i) * p.rank : p.u, take);
           }
         }
-        cp_async_commit();
-        if (it >= C::kLag) {
-          cp_async_wait<C::kLag>();
-          fence_async_shared();
-          mbar_arrive(full((it - C::kLag) % C::kStages));
-        }
+        cp_async_arrive(full(s));
       }
-      cp_async_wait<0>();
-      if (ok) {
-        fence_async_shared();
-        for (int it = max(0, total - C::kLag); it < total; ++it) mbar_arrive(full(it % C::kStages));
-      }
-    } else if (warp == 8) {
+      cp_async_wait_all();
+    } else if (warp == kMmaWarp) {
       // ---- tensor cores ----
       bool ok = true;
       for (int it = 0; it < n1; ++it) {
         const int s = it % C::kStages;
         if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x33))) break;
+        fence_async_shared();
         tc_fence_after_sync();
         const uint32_t a = ring + s * C::kStageBytes, b = a + kRowsBytes;
 #pragma unroll
@@ -302,6 +307,7 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
         const int it = n1 + j, s = it % C::kStages, b = j & 1;
         if (j >= 2 && !(ok = mbar_wait(wctx, out_free(b), ((j >> 1) - 1) & 1, 0x35))) break;
         if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x36))) break;
+        fence_async_shared();
         tc_fence_after_sync();
         const uint32_t w = ring + s * C::kStageBytes + kRowsBytes;
         const uint32_t d = tmem + C::kOut + b * kChunk;
@@ -344,28 +350,45 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
           __syncwarp();
           if (lane < S) mbar_arrive_cluster(bar_parts, lane);
           ok = mbar_wait_cluster(wctx, bar_parts, 0, 0x38);
+          // CTA c adds up the c-th part of the cluster's sums and writes it back to all of them, where only it has read
+          if (ok) {
+            const int all = q.rank16 / 4 * kTile;   // 16-byte pieces
+            for (int e = all / S * rank + threadIdx.x; e < all / S * (rank + 1); e += kEpiWarps * 32) {
+              float4 part[kMaxCluster];
+#pragma unroll
+              for (int c = 0; c < kMaxCluster; ++c)
+                if (c < S) part[c] = ld_shared_cluster_f4(cluster_map_shared(exchange + e * 16, c));
+              float4 sum = part[0];
+#pragma unroll
+              for (int c = 1; c < kMaxCluster; ++c)
+                if (c < S) {
+                  sum.x += part[c].x;
+                  sum.y += part[c].y;
+                  sum.z += part[c].z;
+                  sum.w += part[c].w;
+                }
+#pragma unroll
+              for (int c = 0; c < kMaxCluster; ++c)
+                if (c < S) st_shared_cluster_f4(cluster_map_shared(exchange + e * 16, c), sum);
+            }
+            __syncwarp();
+            if (lane < S) mbar_arrive_cluster(bar_total, lane);
+            ok = mbar_wait_cluster(wctx, bar_total, 0, 0x3b);
+          }
         }
       }
       if (ok) {
         for (int b = 0; b < blocks; ++b) {
           uint32_t x[16];
           if (S > 1) {
-            float sum[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum[i] = 0.f;
-            for (int c = 0; c < S; ++c) {
-              const uint32_t from = cluster_map_shared(exchange, c);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float4 v = ld_shared_cluster_f4(from + ((b * 4 + i) * kTile + r) * 16);
-                sum[4 * i] += v.x;
-                sum[4 * i + 1] += v.y;
-                sum[4 * i + 2] += v.z;
-                sum[4 * i + 3] += v.w;
-              }
+            for (int i = 0; i < 4; ++i) {
+              const uint4 v = ld_shared_v4(exchange + ((b * 4 + i) * kTile + r) * 16);
+              x[4 * i] = v.x;
+              x[4 * i + 1] = v.y;
+              x[4 * i + 2] = v.z;
+              x[4 * i + 3] = v.w;
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(sum[i]);
             tmem_st16(lanes + b * 16, x);
           } else {
             tmem_ld(lanes + b * 16, x);
@@ -465,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
   if (S > 1) cluster_sync();   // (nobody reads this CTA's partial sums any more)
   else __syncthreads();
   tc_fence_after_sync();
-  if (warp == 8) tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
 }
 
 template <typename T, int RB, bool FWD>
@@ -507,7 +530,6 @@ constexpr int kSlab = 256;
 template <int RB>
 struct GradCfg {
   static constexpr int kStages = RB == 1 ? 2 : 3;
-  static constexpr int kLag = kStages - 1;
   static constexpr int kRows = 64 * kSlab * 2;             // four blocks of 64 rows x 128 bytes
   static constexpr int kPart = RB * kBlockBytes;           // one 16-bit part of the vectors
   static constexpr int kStageBytes = kRows + 2 * kPart;
@@ -557,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full(s), 2 * kProdThreads);
+      mbar_init(full(s), (kEpiWarps + kProdWarps) * 32);
       mbar_init(freed(s), 1);
     }
     mbar_init(bar_sums, 1);
@@ -565,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
     fence_barrier_init();
   }
   grid_dependency_wait();
-  if (warp == 8) {   // (behind the wait: a kernel that still runs may need the columns)
+  if (warp == kMmaWarp) {   // (behind the wait: a kernel that still runs may need the columns)
     tmem_alloc(smem_u32(const_cast<uint32_t*>(words)), C::kTmemCols);
     tmem_relinquish();
   }
@@ -584,40 +606,32 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
   };
   float up = 1.f;
 
-  if (warp >= 4 && warp < 8) {
+  if (warp >= kEpiWarps && warp < kMmaWarp) {
     // ---- copies: a warp takes every fourth row, a lane 16 bytes of it ----
-    const int w = warp - 4;
+    const int w = warp - kEpiWarps;
     const int64_t col = col0 + lane * 8;
     const bool in_width = col < width;
     const T* src = rows + (in_width ? col : 0);
-    const uint32_t dst0 = ring + (lane >> 3) * kBlockBytes;
-    bool ok = true;
+    const uint32_t dst0 = ring + (lane >> 3) * kBlockBytes + w * 128;
+    // (row w + 4 i: its swizzle is (w + 4 i) & 7)
+    const uint32_t even = ((lane & 7) ^ w) << 4, odd = ((lane & 7) ^ (w + 4)) << 4;
     int32_t mine = n > 0 ? row_at(chunk0, w + 4 * (lane & 15)) : -1;   // lane i < 16: row w + 4 i
 #pragma unroll 1
     for (int it = 0; it < n; ++it) {
       const int s = it % C::kStages;
-      if (it >= C::kStages && !(ok = mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x41))) break;
+      if (it >= C::kStages && !mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x41)) break;
       const int32_t now = mine;
       if (it + 1 < n) mine = row_at(chunk0 + it + 1, w + 4 * (lane & 15));
+      const uint32_t dst = dst0 + s * C::kStageBytes;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int32_t row = __shfl_sync(0xffffffffu, now, i);
-        const int r = w + 4 * i;
-        cp_async16(dst0 + s * C::kStageBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4), src + (row >= 0 ? row : 0) * ld,
-                   in_width && row >= 0);
+        const bool take = in_width && row >= 0;
+        cp_async16(dst + i * 512 + (i & 1 ? odd : even), take ? src + row * ld : rows, take);
       }
-      cp_async_commit();
-      if (it >= C::kLag) {
-        cp_async_wait<C::kLag>();
-        fence_async_shared();
-        mbar_arrive(full((it - C::kLag) % C::kStages));
-      }
+      cp_async_arrive(full(s));
     }
-    cp_async_wait<0>();
-    if (ok) {
-      fence_async_shared();
-      for (int it = max(0, n - C::kLag); it < n; ++it) mbar_arrive(full(it % C::kStages));
-    }
+    cp_async_wait_all();
   } else if (warp < 4) {
     // ---- vectors: a thread takes 8 ranks of every (16 / RB)-th row ----
     const int t = threadIdx.x;
@@ -686,6 +700,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
     for (int it = 0; it < n; ++it) {
       const int s = it % C::kStages;
       if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x43))) break;
+      fence_async_shared();
       tc_fence_after_sync();
       const uint32_t a = ring + s * C::kStageBytes, b = a + C::kRows;
 #pragma unroll
@@ -768,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
   if (S > 1) cluster_sync();   // (nobody reads this CTA's sums any more)
   else __syncthreads();
   tc_fence_after_sync();
-  if (warp == 8) tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
 }
 
 template <typename T, int RB>
