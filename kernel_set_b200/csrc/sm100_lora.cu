@@ -6,12 +6,12 @@
 // (in rank order, so all CTAs hold the same bits), and each CTA gives its slice of the outputs. The
 // inner vectors never leave the SM, there is one launch, and while the partial sums are exchanged the rows of y0 and V's
 // tiles are already on their way: both phases draw on one ring of shared-memory stages.
-//   warps 0-3   epilogue: a thread per row. Partial sums out of tensor memory, exchange, split into two 16-bit numbers,
+//   warps 0-7   epilogue: two threads per row. Partial sums out of tensor memory, exchange, split into two 16-bit numbers,
 //               back into tensor memory as the second product's A operand; then y0 + c D, in the stage that holds y0's tile,
-//               and out in whole 128-byte row segments
-//   warps 4-7   producer: cp.async of 16 bytes. Rows are gathered by number, tails come as zeros, and neither
+//               and out in 64-byte row segments
+//   warps 8-11  producer: cp.async of 16 bytes. Rows are gathered by number, tails come as zeros, and neither
 //               needs a tensor map (the smallest calls are bound by the host's path)
-//   warp 8      tcgen05.mma: M 128 (rows) x N rank, then M 128 x N 64 (outputs) with K = rank, twice (high and low part)
+//   warp 12     tcgen05.mma: M 128 (rows) x N rank, then M 128 x N 64 (outputs) with K = rank, twice (high and low part)
 // Bound by memory: rows * (d_in + 2 d_out) elements are moved, 2 rank operations for each; the legacy tensor path would be the bound
 // from rank 32 on.
 #include <algorithm>
@@ -31,24 +31,28 @@ constexpr int kTile = kLoraTile;
 constexpr int kChunk = 64;                         // columns of a stage: 128 bytes
 constexpr int kRowsBytes = kTile * kChunk * 2;     // rows' part of a stage
 constexpr int kBlockBytes = 64 * kChunk * 2;       // 64 rows x 128 bytes of a factor
-constexpr int kEpiWarps = 4, kProdWarps = 4, kMmaWarp = kEpiWarps + kProdWarps;
+constexpr int kProdWarps = 4;
 constexpr int kProdThreads = kProdWarps * 32;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kMaxCluster = 8;
 
-// RB: 64-rank blocks (rank <= 64 RB).
-template <int RB>
+// RC: 0 rank <= 32, 1 rank <= 64, 2 rank <= 128. Two CTAs per SM up to rank 64 (one's epilogue under the other's copies).
+template <int RC>
 struct TileCfg {
-  static constexpr int kStages = RB == 1 ? 3 : 4;
+  static constexpr int kRanks = 32 << RC;
+  static constexpr int RB = RC == 2 ? 2 : 1;           // 64-rank blocks
+  static constexpr int kStages = RC == 1 ? 3 : 4;
+  static constexpr int kEpiWarps = 8, kMmaWarp = kEpiWarps + kProdWarps;
+  static constexpr int kThreads = (kMmaWarp + 1) * 32;
   static constexpr int kStageBytes = kRowsBytes + RB * kBlockBytes;
-  static constexpr int kExchange = kTile * 64 * RB * 4;
-  static constexpr int kLo = 64 * RB;               // tensor memory: sums / high part, low part, two output buffers
+  static constexpr int kExchange = kTile * kRanks * 4;
+  static constexpr int kHi = 64 * RB;                  // tensor memory: sums, high part, low part, two output buffers
+  static constexpr int kLo = kHi + 32 * RB;
   static constexpr int kOut = kLo + 32 * RB;
   static constexpr int kTmemCols = RB == 1 ? 256 : 512;
   static constexpr int kPerSm = RB == 1 ? 2 : 1;
   static_assert(kOut + 2 * kChunk <= kTmemCols, "tensor memory layout");
   static constexpr int kBars = 3 * kStages + 8;
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + kExchange + kTile * 4 + 8 * kBars + 64;
+  static constexpr int kSmem = kStages * kStageBytes + kExchange + kTile * 4 + 8 * kBars + 64;
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory");
 };
 
@@ -103,15 +107,6 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-
 // The largest of the warp's values.
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -127,13 +122,46 @@ struct TileParams {
   int cluster;
 };
 
-template <typename T, int RB, bool FWD>
-__global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kernel(const __grid_constant__ TileParams q) {
-  using C = TileCfg<RB>;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// CTA `rank` of S adds up its part of the cluster's sums, in rank order, and writes the totals back to all of them, where only it has
+// read. A thread has eight 16-byte loads from other SMs in flight.
+template <int S, int THREADS>
+__device__ __forceinline__ void reduce_scatter(uint32_t exchange, int pieces, int rank) {
+  constexpr int kAtOnce = kMaxCluster / S;
+  const int end = pieces / S * (rank + 1);
+  for (int e0 = pieces / S * rank + threadIdx.x; e0 < end; e0 += kAtOnce * THREADS) {
+    float4 part[kAtOnce][S];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+      for (int c = 0; c < S; ++c)
+        if (e0 + u * THREADS < end) part[u][c] = ld_shared_cluster_f4(cluster_map_shared(exchange + (e0 + u * THREADS) * 16, c));
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (e0 + u * THREADS >= end) continue;
+      float4 sum = part[u][0];
+#pragma unroll
+      for (int c = 1; c < S; ++c) {
+        sum.x += part[u][c].x;
+        sum.y += part[u][c].y;
+        sum.z += part[u][c].z;
+        sum.w += part[u][c].w;
+      }
+#pragma unroll
+      for (int c = 0; c < S; ++c) st_shared_cluster_f4(cluster_map_shared(exchange + (e0 + u * THREADS) * 16, c), sum);
+    }
+  }
+}
+
+template <typename T, int RC, bool FWD>
+__global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lora_tile_kernel(const __grid_constant__ TileParams q) {
+  using C = TileCfg<RC>;
+  constexpr int RB = C::RB;
+  extern __shared__ __align__(1024) unsigned char smem[];
   const LoraPass& p = q.p;
-  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const uint32_t ring = smem_u32(smem);
+  const uint32_t ring = smem_u32(smem);   // (1024-byte aligned: there is no static shared memory)
   const uint32_t exchange = ring + C::kStages * C::kStageBytes;
   int32_t* row_of = reinterpret_cast<int32_t*>(smem + C::kStages * C::kStageBytes + C::kExchange);
   uint64_t* bar_mem = reinterpret_cast<uint64_t*>(row_of + kTile);
@@ -157,21 +185,24 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(full(s), kProdThreads);
       mbar_init(free1(s), 1);
-      mbar_init(free2(s), kEpiWarps);
+      mbar_init(free2(s), C::kEpiWarps);
     }
     mbar_init(bar_sums, 1);
-    mbar_init(bar_inner, kEpiWarps * 32);
-    mbar_init(bar_parts, static_cast<uint32_t>(S) * kEpiWarps);
-    mbar_init(bar_total, static_cast<uint32_t>(S) * kEpiWarps);
+    mbar_init(bar_inner, C::kEpiWarps * 32);
+    mbar_init(bar_parts, static_cast<uint32_t>(S) * C::kEpiWarps);
+    mbar_init(bar_total, static_cast<uint32_t>(S) * C::kEpiWarps);
     for (int b = 0; b < 2; ++b) {
       mbar_init(out_full(b), 1);
-      mbar_init(out_free(b), kEpiWarps);
+      mbar_init(out_free(b), C::kEpiWarps);
     }
     words[1] = 0u;
     fence_barrier_init();
   }
+  __syncwarp();
+  bool joined = S == 1;            // (waited for the other CTAs' barriers to be initialised)
+  if (!joined) cluster_arrive();
   grid_dependency_wait();
-  if (warp == kMmaWarp) {   // (behind the wait: a kernel that still runs may need the columns)
+  if (warp == C::kMmaWarp) {   // (behind the wait: a kernel that still runs may need the columns)
     tmem_alloc(smem_u32(const_cast<uint32_t*>(words)), C::kTmemCols);
     tmem_relinquish();
   }
@@ -182,11 +213,14 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
       words[3] = static_cast<uint32_t>(f.count);
       words[4] = static_cast<uint32_t>(f.place);
     }
-    for (int i = lane; i < kTile; i += 32) row_of[i] = i < f.count ? static_cast<int32_t>(lora_row(p.ids, f.place + i, p.rows)) : -1;
+#pragma unroll
+    for (int i = 0; i < kTile / 32; ++i) {
+      const int r = i * 32 + lane;
+      row_of[r] = r < f.count ? static_cast<int32_t>(lora_row(p.ids, f.place + r, p.rows)) : -1;
+    }
   }
   tc_fence_before_sync();
-  if (S > 1) cluster_sync();   // (the barriers that other CTAs arrive on are initialised)
-  else __syncthreads();
+  __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = words[0];
   const int adapter = static_cast<int>(words[2]);
@@ -205,20 +239,27 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
     if (p.out != p.base) {
       const int64_t c0 = static_cast<int64_t>(out0) * kChunk;
       const int64_t c1 = min(p.d_out, c0 + static_cast<int64_t>(n2) * kChunk);
-      for (int r = warp; r < count; r += kThreads / 32) {
+      for (int r = warp; r < count; r += C::kThreads / 32) {
         const int64_t row = row_of[r];
         if (row < 0) continue;
         const T* src = static_cast<const T*>(p.base) + row * p.ld_base;
         T* dst = static_cast<T*>(p.out) + row * p.ld_out;
-        for (int64_t c = c0 + lane * 8; c < c1; c += 256)
-          *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+        for (int64_t c = c0 + lane * 8; c < c1; c += 8 * 256) {
+          uint4 v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (c + u * 256 < c1) v[u] = *reinterpret_cast<const uint4*>(src + c + u * 256);
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (c + u * 256 < c1) __stcs(reinterpret_cast<uint4*>(dst + c + u * 256), v[u]);
+        }
       }
     }
   } else if (adapter >= 0) {
     const int total = n1 + n2;
-    if (warp >= kEpiWarps && warp < kMmaWarp) {
+    if (warp >= C::kEpiWarps && warp < C::kMmaWarp) {
       // ---- producer ----
-      const int t = threadIdx.x - kEpiWarps * 32;
+      const int t = threadIdx.x - C::kEpiWarps * 32;
       const int c8 = t & 7, r0 = t >> 3;                         // rows' part: 16 bytes of the rows r0 + 16 i
       const int j8 = t % (8 * RB), i0 = t / (8 * RB);            // 64 rows of `rank` columns: rows i0 + 16 / RB * i
       const T* u = static_cast<const T*>(p.u) + static_cast<int64_t>(adapter) * p.rank * p.d_in;
@@ -282,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
         cp_async_arrive(full(s));
       }
       cp_async_wait_all();
-    } else if (warp == kMmaWarp) {
+    } else if (warp == C::kMmaWarp) {
       // ---- tensor cores ----
       bool ok = true;
       for (int it = 0; it < n1; ++it) {
@@ -314,72 +355,52 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
         for (int kk = 0; kk < q.rank16 / 16; ++kk) {
           const uint64_t bd = FWD ? umma_smem_desc_sw128(w + (kk >> 2) * kBlockBytes + (kk & 3) * 32, 16, 1024)
                                   : umma_smem_desc_sw128(w + kk * 16 * 128, kBlockBytes, 1024);
-          umma_f16_tmem_a_elect(d, tmem + kk * 8, bd, q.idesc2, kk > 0 ? 1u : 0u);
+          umma_f16_tmem_a_elect(d, tmem + C::kHi + kk * 8, bd, q.idesc2, kk > 0 ? 1u : 0u);
           umma_f16_tmem_a_elect(d, tmem + C::kLo + kk * 8, bd, q.idesc2, 1u);
         }
         tc_commit_elect(out_full(b));
       }
-    } else if (warp < 4) {
-      // ---- epilogue: thread = row ----
-      const int r = threadIdx.x;
-      const int32_t row = row_of[r];
-      const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) << 21);
+    } else {
+      // ---- epilogue: a thread per row and half (of the ranks, of a chunk's columns) ----
+      const int quarter = warp & 3, half = warp >> 2;
+      const int r = quarter * 32 + lane;
+      const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter) << 21);
       const float s = __ldg(p.scales + adapter);
       const int blocks = q.rank16 / 16;
+      if (!joined) cluster_wait();
+      joined = true;
       bool ok = n1 == 0 || mbar_wait_long(wctx, bar_sums, 0, 0x37);
-      float most = 0.f, down, up;
-      float* inner = p.inner != nullptr && rank == 0 && row >= 0 ? p.inner + static_cast<int64_t>(row) * p.rank : nullptr;
-      const float inner_scale = p.scale_inner ? s : 1.f;
-      if (ok) {
-        tc_fence_after_sync();
-        if (S > 1) {
-          // 16 bytes of rank 4j.. of row r at exchange + (j * 128 + r) * 16
-          for (int b = 0; b < blocks; ++b) {
-            uint32_t x[16];
-            if (n1 > 0) {
-              tmem_ld(lanes + b * 16, x);
-              tmem_wait_ld(x);
-            } else {
+      tc_fence_after_sync();
+      if (ok && S > 1) {
+        // ranks 4 j .. of row r at exchange + (j * 128 + r) * 16
+        for (int b = half; b < blocks; b += 2) {
+          uint32_t x[16];
+          if (n1 > 0) {
+            tmem_ld(lanes + b * 16, x);
+            tmem_wait_ld(x);
+          } else {
 #pragma unroll
-              for (int i = 0; i < 16; ++i) x[i] = 0u;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              st_shared_v4(exchange + ((b * 4 + i) * kTile + r) * 16, x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            for (int i = 0; i < 16; ++i) x[i] = 0u;
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            st_shared_v4(exchange + ((b * 4 + i) * kTile + r) * 16, x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        }
+        __syncwarp();
+        if (lane < S) mbar_arrive_cluster(bar_parts, lane);
+        ok = mbar_wait_cluster(wctx, bar_parts, 0, 0x38);
+        if (ok) {
+          const int pieces = q.rank16 / 4 * kTile;
+          if (S == 2) reduce_scatter<2, C::kEpiWarps * 32>(exchange, pieces, rank);
+          else if (S == 4) reduce_scatter<4, C::kEpiWarps * 32>(exchange, pieces, rank);
+          else reduce_scatter<8, C::kEpiWarps * 32>(exchange, pieces, rank);
           __syncwarp();
-          if (lane < S) mbar_arrive_cluster(bar_parts, lane);
-          ok = mbar_wait_cluster(wctx, bar_parts, 0, 0x38);
-          // CTA c adds up the c-th part of the cluster's sums and writes it back to all of them, where only it has read
-          if (ok) {
-            const int all = q.rank16 / 4 * kTile;   // 16-byte pieces
-            for (int e = all / S * rank + threadIdx.x; e < all / S * (rank + 1); e += kEpiWarps * 32) {
-              float4 part[kMaxCluster];
-#pragma unroll
-              for (int c = 0; c < kMaxCluster; ++c)
-                if (c < S) part[c] = ld_shared_cluster_f4(cluster_map_shared(exchange + e * 16, c));
-              float4 sum = part[0];
-#pragma unroll
-              for (int c = 1; c < kMaxCluster; ++c)
-                if (c < S) {
-                  sum.x += part[c].x;
-                  sum.y += part[c].y;
-                  sum.z += part[c].z;
-                  sum.w += part[c].w;
-                }
-#pragma unroll
-              for (int c = 0; c < kMaxCluster; ++c)
-                if (c < S) st_shared_cluster_f4(cluster_map_shared(exchange + e * 16, c), sum);
-            }
-            __syncwarp();
-            if (lane < S) mbar_arrive_cluster(bar_total, lane);
-            ok = mbar_wait_cluster(wctx, bar_total, 0, 0x3b);
-          }
+          if (lane < S) mbar_arrive_cluster(bar_total, lane);
+          ok = mbar_wait_cluster(wctx, bar_total, 0, 0x3b);
         }
       }
       if (ok) {
-        for (int b = 0; b < blocks; ++b) {
-          uint32_t x[16];
+        const auto sums_of = [&](int b, uint32_t (&x)[16]) {
           if (S > 1) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -389,22 +410,47 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
               x[4 * i + 2] = v.z;
               x[4 * i + 3] = v.w;
             }
-            tmem_st16(lanes + b * 16, x);
           } else {
             tmem_ld(lanes + b * 16, x);
             tmem_wait_ld(x);
           }
+        };
+        const int32_t row = row_of[r];
+        float most = 0.f, down, up;
+        for (int b = 0; b < blocks; ++b) {
+          uint32_t x[16];
+          sums_of(b, x);
 #pragma unroll
           for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(__uint_as_float(x[i])));
+        }
+        row_scale(most, &down, &up);
+        const float inner_scale = p.scale_inner ? s : 1.f;
+        float* inner = p.inner != nullptr && rank == 0 && row >= 0 ? p.inner + static_cast<int64_t>(row) * p.rank : nullptr;
+        for (int b = half; b < blocks; b += 2) {
+          uint32_t x[16], hi[8], lo[8];
+          sums_of(b, x);
           if (inner != nullptr) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (b * 16 + i < p.rank) inner[b * 16 + i] = inner_scale * __uint_as_float(x[i]);
+            for (int i = 0; i < 16; i += 4)
+              if (b * 16 + i < p.rank)
+                *reinterpret_cast<float4*>(inner + b * 16 + i) =
+                    make_float4(inner_scale * __uint_as_float(x[i]), inner_scale * __uint_as_float(x[i + 1]),
+                                inner_scale * __uint_as_float(x[i + 2]), inner_scale * __uint_as_float(x[i + 3]));
           }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float f0 = __uint_as_float(x[2 * i]) * down, f1 = __uint_as_float(x[2 * i + 1]) * down;
+            hi[i] = Pair<T>::pack(f0, f1);
+            const float2 h = Pair<T>::unpack(hi[i]);
+            lo[i] = Pair<T>::pack(f0 - h.x, f1 - h.y);
+          }
+          tmem_st8(lanes + C::kHi + b * 8, hi);
+          tmem_st8(lanes + C::kLo + b * 8, lo);
         }
         tmem_wait_st();
-        row_scale(most, &down, &up);
-        if (p.most_g != nullptr && rank == 0) {
+        tc_fence_before_sync();
+        mbar_arrive(bar_inner);
+        if (p.most_g != nullptr && rank == 0 && half == 0) {
           float most_h = 0.f;
           if (row >= 0)
             for (int i = 0; i < p.rank; i += 4) {
@@ -413,31 +459,23 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
             }
           most_h = warp_max(most_h);
           const float most_g = warp_max(row >= 0 ? most * fabsf(inner_scale) : 0.f);
-          if (lane == 0 && warp * 32 < count) {
-            const int64_t at = place + warp * 32;
-            p.most_g[at] = most_g;
-            p.most_h[at] = most_h;
+          if (lane == 0 && quarter * 32 < count) {
+            p.most_g[place + quarter * 32] = most_g;
+            p.most_h[place + quarter * 32] = most_h;
           }
         }
-        for (int b = 0; b < blocks; ++b) {
-          uint32_t x[16], hi[8], lo[8];
-          tmem_ld(lanes + b * 16, x);
-          tmem_wait_ld(x);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float f0 = __uint_as_float(x[2 * i]) * down, f1 = __uint_as_float(x[2 * i + 1]) * down;
-            hi[i] = Pair<T>::pack(f0, f1);
-            const float2 h = Pair<T>::unpack(hi[i]);
-            lo[i] = Pair<T>::pack(f0 - h.x, f1 - h.y);
-          }
-          tmem_st8(lanes + b * 8, hi);
-          tmem_st8(lanes + C::kLo + b * 8, lo);
-        }
-        tmem_wait_st();
-        tc_fence_before_sync();
-        mbar_arrive(bar_inner);
+        // second product: y0 + c D in the stage that holds y0, then out: rows quarter * 32 + i * 8 + lane % 8, 64 bytes of each
         const float c = s * up;
-        T* out = static_cast<T*>(p.out);
+        const int piece = half * 4 + (lane >> 3);
+        T* dst[4];
+        uint32_t have = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int32_t to = row_of[quarter * 32 + i * 8 + (lane & 7)];
+          if (to >= 0) have |= 1u << i;
+          dst[i] = static_cast<T*>(p.out) + (to >= 0 ? to : 0) * p.ld_out + static_cast<int64_t>(out0) * kChunk + piece * 8;
+        }
+#pragma unroll 1
         for (int j = 0; j < n2; ++j) {
           const int it = n1 + j, st = it % C::kStages, b = j & 1;
           if (!mbar_wait(wctx, out_full(b), (j >> 1) & 1, 0x39)) break;
@@ -445,18 +483,18 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
           tc_fence_after_sync();
           const uint32_t tile = ring + st * C::kStageBytes;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t d[32];
-            tmem_ld(lanes + C::kOut + b * kChunk + half * 32, d);
+          for (int part = 0; part < 2; ++part) {
+            uint32_t d[16];
+            tmem_ld(lanes + C::kOut + b * kChunk + half * 32 + part * 16, d);
             tmem_wait_ld(d);
-            if (half == 1) {
+            if (part == 1) {
               tc_fence_before_sync();
               __syncwarp();
               if (lane == 0) mbar_arrive(out_free(b));
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t at = tile + r * 128 + (((half * 4 + i) ^ (r & 7)) << 4);
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t at = tile + r * 128 + (((half * 4 + part * 2 + i) ^ (r & 7)) << 4);
               const uint4 y0 = ld_shared_v4(at);
               uint32_t y[4] = {y0.x, y0.y, y0.z, y0.w};
 #pragma unroll
@@ -469,13 +507,13 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
             }
           }
           __syncwarp();
-          const int64_t col = static_cast<int64_t>(out0 + j) * kChunk + (lane & 7) * 8;
+          const bool in_width = static_cast<int64_t>(out0 + j) * kChunk + piece * 8 < p.d_out;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int rr = warp * 32 + i * 4 + (lane >> 3);
-            const uint4 y = ld_shared_v4(tile + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-            const int64_t dst_row = row_of[rr];
-            if (dst_row >= 0 && col < p.d_out) __stcs(reinterpret_cast<uint4*>(out + dst_row * p.ld_out + col), y);
+          for (int i = 0; i < 4; ++i) {
+            const int rr = quarter * 32 + i * 8 + (lane & 7);
+            const uint4 y = ld_shared_v4(tile + rr * 128 + ((piece ^ (rr & 7)) << 4));
+            if (in_width && (have >> i & 1u)) __stcs(reinterpret_cast<uint4*>(dst[i]), y);
+            dst[i] += kChunk;
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(free2(st));
@@ -485,15 +523,19 @@ __global__ void __launch_bounds__(kThreads, TileCfg<RB>::kPerSm) lora_tile_kerne
   }
   __syncwarp();
   tc_fence_before_sync();
-  if (S > 1) cluster_sync();   // (nobody reads this CTA's partial sums any more)
-  else __syncthreads();
+  if (S > 1) {
+    if (!joined) cluster_wait();
+    cluster_sync();   // (nobody reads this CTA's partial sums any more)
+  } else {
+    __syncthreads();
+  }
   tc_fence_after_sync();
-  if (warp == kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == C::kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
 }
 
-template <typename T, int RB, bool FWD>
+template <typename T, int RC, bool FWD>
 ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, cudaStream_t stream) {
-  using C = TileCfg<RB>;
+  using C = TileCfg<RC>;
   static std::mutex mu;
   static bool done[64] = {};
   int dev = 0;
@@ -501,13 +543,13 @@ ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, c
   {
     std::lock_guard<std::mutex> lock(mu);
     if (dev >= 0 && dev < 64 && !done[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(lora_tile_kernel<T, RB, FWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+      const cudaError_t e = cudaFuncSetAttribute(lora_tile_kernel<T, RC, FWD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
       if (e != cudaSuccess) return cuda_status(e, where);
       done[dev] = true;
     }
   }
-  launch_programmatic_cluster(lora_tile_kernel<T, RB, FWD>, static_cast<unsigned>(tiles * q.cluster), static_cast<unsigned>(q.cluster),
-                              true, kThreads, C::kSmem, stream, q);
+  launch_programmatic_cluster(lora_tile_kernel<T, RC, FWD>, static_cast<unsigned>(tiles * q.cluster), static_cast<unsigned>(q.cluster),
+                              true, C::kThreads, C::kSmem, stream, q);
   KSB_CHECK_LAUNCH(where);
   return KS_SUCCESS;
 }
@@ -530,6 +572,8 @@ constexpr int kSlab = 256;
 template <int RB>
 struct GradCfg {
   static constexpr int kStages = RB == 1 ? 2 : 3;
+  static constexpr int kVecWarps = 4, kMmaWarp = kVecWarps + kProdWarps;
+  static constexpr int kThreads = (kMmaWarp + 1) * 32;
   static constexpr int kRows = 64 * kSlab * 2;             // four blocks of 64 rows x 128 bytes
   static constexpr int kPart = RB * kBlockBytes;           // one 16-bit part of the vectors
   static constexpr int kStageBytes = kRows + 2 * kPart;
@@ -551,7 +595,7 @@ struct GradParams {
 };
 
 template <typename T, int RB>
-__global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_grad_kernel(const __grid_constant__ GradParams q) {
+__global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lora_weight_grad_kernel(const __grid_constant__ GradParams q) {
   using C = GradCfg<RB>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const LoraWeightGrad& p = q.p;
@@ -579,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full(s), (kEpiWarps + kProdWarps) * 32);
+      mbar_init(full(s), (C::kVecWarps + kProdWarps) * 32);
       mbar_init(freed(s), 1);
     }
     mbar_init(bar_sums, 1);
@@ -587,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
     fence_barrier_init();
   }
   grid_dependency_wait();
-  if (warp == kMmaWarp) {   // (behind the wait: a kernel that still runs may need the columns)
+  if (warp == C::kMmaWarp) {   // (behind the wait: a kernel that still runs may need the columns)
     tmem_alloc(smem_u32(const_cast<uint32_t*>(words)), C::kTmemCols);
     tmem_relinquish();
   }
@@ -606,9 +650,9 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
   };
   float up = 1.f;
 
-  if (warp >= kEpiWarps && warp < kMmaWarp) {
+  if (warp >= C::kVecWarps && warp < C::kMmaWarp) {
     // ---- copies: a warp takes every fourth row, a lane 16 bytes of it ----
-    const int w = warp - kEpiWarps;
+    const int w = warp - C::kVecWarps;
     const int64_t col = col0 + lane * 8;
     const bool in_width = col < width;
     const T* src = rows + (in_width ? col : 0);
@@ -750,7 +794,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
   };
   if (is_a) {
     T* out = static_cast<T*>(p.d_a) + factor;
-    for (int e = threadIdx.x; e < p.rank * (cols / 8); e += kThreads) {
+    for (int e = threadIdx.x; e < p.rank * (cols / 8); e += C::kThreads) {
       const int j = e / (cols / 8), m = rank * cols + (e % (cols / 8)) * 8;
       if (col0 + m >= width) continue;
       float f[8] = {};
@@ -764,7 +808,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
     }
   } else {
     T* out = static_cast<T*>(p.d_b) + factor;
-    for (int e = threadIdx.x; e < p.rank / 8 * cols; e += kThreads) {
+    for (int e = threadIdx.x; e < p.rank / 8 * cols; e += C::kThreads) {
       const int j = e / cols * 8, m = rank * cols + e % cols;
       if (col0 + m >= width) continue;
       float f[8] = {};
@@ -783,7 +827,7 @@ __global__ void __launch_bounds__(kThreads, GradCfg<RB>::kPerSm) lora_weight_gra
   if (S > 1) cluster_sync();   // (nobody reads this CTA's sums any more)
   else __syncthreads();
   tc_fence_after_sync();
-  if (warp == kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
+  if (warp == C::kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
 }
 
 template <typename T, int RB>
@@ -802,7 +846,7 @@ ks_status_t launch_grad(const char* where, const GradParams& q, int64_t items, c
     }
   }
   launch_programmatic_cluster(lora_weight_grad_kernel<T, RB>, static_cast<unsigned>(items * q.cluster), static_cast<unsigned>(q.cluster),
-                              true, kThreads, C::kSmem, stream, q);
+                              true, C::kThreads, C::kSmem, stream, q);
   KSB_CHECK_LAUNCH(where);
   return KS_SUCCESS;
 }
@@ -811,7 +855,7 @@ ks_status_t launch_grad(const char* where, const GradParams& q, int64_t items, c
 
 bool lora_tile_takes(const LoraPass& p) {
   const auto rows16 = [](const void* m, int64_t ld) { return aligned16(m) && ld % 8 == 0; };
-  return p.rank % 8 == 0 && p.rank <= 128 && p.d_in % 8 == 0 && p.d_out % 8 == 0 && aligned16(p.u) && aligned16(p.v) &&
+  return p.rank % 8 == 0 && p.rank <= 128 && p.d_in % 8 == 0 && p.d_out % 8 == 0 && aligned16(p.u) && aligned16(p.v) && aligned16(p.inner) &&
          rows16(p.in, p.ld_in) && rows16(p.base, p.ld_base) && rows16(p.out, p.ld_out);
 }
 
@@ -831,10 +875,12 @@ ks_status_t lora_tile_pass(const char* where, const LoraPass& p, bool forward, k
   while (s < kMaxCluster && filled * s * 2 <= room) s *= 2;
   q.cluster = s;
   if (tiles * s > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
-#define KSB_LORA_TILE(T)                                                                                                         \
-  (forward ? (wide ? launch_tile<T, 2, true>(where, q, tiles, stream) : launch_tile<T, 1, true>(where, q, tiles, stream))        \
-           : (wide ? launch_tile<T, 2, false>(where, q, tiles, stream) : launch_tile<T, 1, false>(where, q, tiles, stream)))
-  return dtype == KS_DTYPE_F16 ? KSB_LORA_TILE(__half) : KSB_LORA_TILE(__nv_bfloat16);
+#define KSB_LORA_TILE(T, FWD)                                                      \
+  (p.rank <= 32   ? launch_tile<T, 0, FWD>(where, q, tiles, stream)                \
+   : p.rank <= 64 ? launch_tile<T, 1, FWD>(where, q, tiles, stream)                \
+                  : launch_tile<T, 2, FWD>(where, q, tiles, stream))
+  if (dtype == KS_DTYPE_F16) return forward ? KSB_LORA_TILE(__half, true) : KSB_LORA_TILE(__half, false);
+  return forward ? KSB_LORA_TILE(__nv_bfloat16, true) : KSB_LORA_TILE(__nv_bfloat16, false);
 #undef KSB_LORA_TILE
 }
 
