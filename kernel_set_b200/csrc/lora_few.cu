@@ -1,16 +1,17 @@
-// Low-rank adapters for single tokens: y = y0 + s B (A x) for up to 8 rows of an adapter at a time.
+// Low-rank adapters for single tokens and short prompts: y = y0 + s B (A x) for 8, 16 or 32 rows of an adapter at a time.
 //
 // What counts here is latency: an adapter of rank 16 beside a 4096 x 4096 projection is 256 KB. One launch does both products. A
-// cluster of CTAs has an item (up to 8 rows of one adapter): each takes a slice of K, leaves its partial sums [rank x 8] in
+// cluster of CTAs has an item (up to 32 rows of one adapter): each takes a slice of K, leaves its partial sums [rank x rows] in
 // every CTA's shared memory, and behind one cluster barrier each has the whole inner vectors, added in rank order, and
 // computes a slice of the outputs. With few items several clusters share one: each does the first product again (A comes from
 // L2) and gives a part of the outputs. B's slice is asked into L2 at the start.
 //
-// Products by mma.m16n8k16 with the factor as the 16-row operand and the rows as the 8 columns; its order of k inside a block of
+// Products by mma.m16n8k16 with the factor as the 16-row operand and 8 rows as the columns; its order of k inside a block of
 // 32 is changed so that a lane's four pairs are 16 adjacent bytes, and its order of rows in the second product so that a
 // lane ends up with 8 adjacent outputs of two rows. The inner vectors enter as a high and a low 16-bit part, scaled per row.
-#include <algorithm>
+#include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "lora_tiles.cuh"
 #include "sm100_host.cuh"
@@ -21,7 +22,6 @@ namespace ksb {
 namespace sm100 {
 namespace {
 
-constexpr int kFew = 8;                // rows of an item
 constexpr int kFewWarps = 8;
 constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kFewCluster = 8;
@@ -42,39 +42,52 @@ __device__ __forceinline__ uint4 load16(const void* p, bool take) {
   return take ? __ldg(static_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
 }
 
-// RT: 16-rank tiles.
-template <typename T, int RT>
-__global__ void __launch_bounds__(kFewThreads, RT <= 2 ? 3 : (RT <= 4 ? 2 : 1)) lora_few_kernel(const __grid_constant__ LoraPass p, int S, int parts) {
-  constexpr int kRanks = RT * 16;
-  constexpr int kBlocks = (RT + 1) / 2;                       // 32-rank blocks of the second product
-  constexpr int kH = kBlocks * 32 * kFew;
-  constexpr int kSums = RT <= 4 ? kFewWarps : kFewWarps / 2;   // (two warps share one at rank 128: 48 KB hold no more)
-  __shared__ __align__(16) float warp_sum[kSums][kRanks * kFew];
-  __shared__ __align__(16) float part_sum[kFewCluster][kRanks * kFew];   // of the cluster's CTAs
-  float* h = &warp_sum[0][0];   // the inner vectors, once the warps' sums have been added up
-  static_assert(kH <= kSums * kRanks * kFew, "shared memory");
+// RT: 16-rank tiles, NT: groups of 8 rows of an item.
+template <int RT, int NT>
+struct FewCfg {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kRanks = RT * 16;
+  static constexpr int kBlocks = (RT + 1) / 2;                          // 32-rank blocks of the second product
+  static constexpr int kElems = kRanks * kRows;                         // of the inner vectors, [rank][row]
+  static constexpr int kSums = RT * NT <= 8 ? kFewWarps : (RT * NT <= 16 ? 4 : 2);   // places for the warps' sums
+  static constexpr int kParts = kSums * kElems * 4;                     // the cluster's sums lie behind them
+  static constexpr int kFrag = kParts + kFewCluster * kElems * 4;       // 16-bit parts of the inner vectors, as operands
+  static constexpr int kUp = kFrag + NT * kBlocks * 32 * 32;            // the rows' scales
+  static constexpr int kSmem = kUp + kRows * 4;
+  static constexpr int kPerSm = RT * NT == 1 ? 3 : (RT <= 4 ? 2 : 1);
+  static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory");
+};
+
+template <typename T, int RT, int NT>
+__global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_kernel(const __grid_constant__ LoraPass p, int S, int parts) {
+  using C = FewCfg<RT, NT>;
+  extern __shared__ __align__(16) unsigned char few_smem[];
+  float* warp_sum = reinterpret_cast<float*>(few_smem);
+  float* part_sum = reinterpret_cast<float*>(few_smem + C::kParts);
+  uint4* frag = reinterpret_cast<uint4*>(few_smem + C::kFrag);          // [group][block][high, low][lane]
+  float* ups = reinterpret_cast<float*>(few_smem + C::kUp);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, s4 = lane & 3;
   const int rank = blockIdx.x % S;
   const int part = (blockIdx.x / S) % parts;
   const int64_t item = blockIdx.x / (S * parts);
   if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (waited for before the first remote store)
   grid_dependency_wait();
-  const TilePlace f = find_tile<kFew>(p.offsets, p.adapters, p.rows, item);
+  const TilePlace f = find_tile<C::kRows>(p.offsets, p.adapters, p.rows, item);
   // outputs of this CTA, in units
   const int64_t units = (p.d_out + kUnit - 1) / kUnit;
   const int slot = part * S + rank;
   const int64_t unit0 = units * slot / (S * parts), unit1 = units * (slot + 1) / (S * parts);
-  const bool work = f.adapter >= 0 && f.adapter < p.adapters;
-  if (!work) {
-    if (f.adapter == p.adapters && p.out != p.base)
-      for (int r = 0; r < f.count; ++r) {
+  if (f.adapter < 0 || f.adapter >= p.adapters) {
+    if (f.adapter == p.adapters && p.out != p.base) {
+      const int64_t end = unit1 * kUnit < p.d_out ? unit1 * kUnit : p.d_out;
+      for (int r = warp; r < f.count; r += kFewWarps) {
         const int64_t row = lora_row(p.ids, f.place + r, p.rows);
         if (row < 0) continue;
-        const int64_t end = unit1 * kUnit < p.d_out ? unit1 * kUnit : p.d_out;
-        for (int64_t c = unit0 * kUnit + threadIdx.x * 8; c < end; c += kFewThreads * 8)
+        for (int64_t c = unit0 * kUnit + lane * 8; c < end; c += 256)
           *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.ld_out + c) =
               *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + row * p.ld_base + c);
       }
+    }
     if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     return;   // (the whole cluster)
   }
@@ -87,20 +100,28 @@ __global__ void __launch_bounds__(kFewThreads, RT <= 2 ? 3 : (RT <= 4 ? 2 : 1)) 
       asm volatile("prefetch.global.L2 [%0];" ::"l"(from + at));
   }
   const float scale = __ldg(p.scales + f.adapter);
-  const int64_t my_row = g < f.count ? lora_row(p.ids, f.place + g, p.rows) : -1;   // row g of the item
-  const T* x = static_cast<const T*>(p.in) + (my_row >= 0 ? my_row : 0) * p.ld_in;
+  const int groups = (f.count + 7) / 8;   // that hold rows
+  int32_t my_row[NT];                     // row g of each group, -1 for none
+  const T* x[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    my_row[n] = n * 8 + g < f.count ? static_cast<int32_t>(lora_row(p.ids, f.place + n * 8 + g, p.rows)) : -1;
+    x[n] = static_cast<const T*>(p.in) + (my_row[n] >= 0 ? my_row[n] : 0) * p.ld_in;
+  }
 
   // ---- first product: blocks of 32 k, warp by warp ----
   const int64_t blocks = (p.d_in + 31) / 32;
   const int64_t block0 = blocks * rank / S, block1 = blocks * (rank + 1) / S;
-  float acc[RT][4];
+  float acc[RT][NT][4];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-  constexpr int kAhead = RT <= 2 ? 2 : 1;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][n][i] = 0.f;
+  constexpr int kAhead = RT <= 2 && NT <= 2 ? 2 : 1;
   for (int64_t blk = block0 + warp; blk < block1; blk += kAhead * kFewWarps) {
-    uint4 xv[kAhead], av[kAhead][RT][2];
+    uint4 xv[kAhead][NT], av[kAhead][RT][2];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int64_t k = (blk + u * kFewWarps) * 32 + s4 * 8;
@@ -113,166 +134,211 @@ __global__ void __launch_bounds__(kFewThreads, RT <= 2 ? 3 : (RT <= 4 ? 2 : 1)) 
           const bool take = in && j < p.rank;
           av[u][t][i] = load16(a + (take ? j * p.d_in + k : 0), take);
         }
-      xv[u] = load16(x + (in ? k : 0), in && my_row >= 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) xv[u][n] = load16(x[n] + (in ? k : 0), in && my_row[n] >= 0);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const uint4 lo = av[u][t][0], hi = av[u][t][1];
-        mma16816<T>(acc[t], lo.x, hi.x, lo.y, hi.y, xv[u].x, xv[u].y);
-        mma16816<T>(acc[t], lo.z, hi.z, lo.w, hi.w, xv[u].z, xv[u].w);
+      for (int n = 0; n < NT; ++n) {
+        if (n >= groups) continue;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const uint4 lo = av[u][t][0], hi = av[u][t][1];
+          mma16816<T>(acc[t][n], lo.x, hi.x, lo.y, hi.y, xv[u][n].x, xv[u][n].y);
+          mma16816<T>(acc[t][n], lo.z, hi.z, lo.w, hi.w, xv[u][n].z, xv[u][n].w);
+        }
       }
   }
-  if (kSums < kFewWarps) {
-    if (warp >= kSums)
+  // the warps' sums: the upper ones leave theirs where the lower ones add their own, until kSums are left
+  const auto sum_at = [&](int w, int t, int n, int i) {
+    return reinterpret_cast<float2*>(warp_sum + w * C::kElems + (t * 16 + g + 8 * i) * C::kRows + n * 8 + 2 * s4);
+  };
+#pragma unroll
+  for (int from = kFewWarps - C::kSums; from >= 0; from -= C::kSums) {
+    if (warp >= from && warp < from + C::kSums) {
+      const int w = warp - from;
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          *reinterpret_cast<float2*>(&warp_sum[warp - kSums][(t * 16 + g + 8 * i) * kFew + 2 * s4]) = make_float2(acc[t][2 * i], acc[t][2 * i + 1]);
-    __syncthreads();
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float2* at = sum_at(w, t, n, i);
+            const float2 other = from < kFewWarps - C::kSums ? *at : make_float2(0.f, 0.f);
+            *at = make_float2(acc[t][n][2 * i] + other.x, acc[t][n][2 * i + 1] + other.y);
+          }
+    }
+    if (from > 0) __syncthreads();
   }
-  if (warp < kSums)
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float2* at = reinterpret_cast<float2*>(&warp_sum[warp][(t * 16 + g + 8 * i) * kFew + 2 * s4]);
-        const float2 other = kSums < kFewWarps ? *at : make_float2(0.f, 0.f);
-        *at = make_float2(acc[t][2 * i] + other.x, acc[t][2 * i + 1] + other.y);
-      }
   if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // (the others have begun)
   __syncthreads();
-  for (int e = threadIdx.x; e < kRanks * kFew; e += kFewThreads) {
-    float v = 0.f;
+  // every CTA's sums to all of the cluster's
+  for (int e = threadIdx.x * 4; e < C::kElems; e += kFewThreads * 4) {
+    float4 v = *reinterpret_cast<const float4*>(warp_sum + e);
 #pragma unroll
-    for (int w = 0; w < kSums; ++w) v += warp_sum[w][e];
-    const uint32_t at = smem_u32(&part_sum[rank][e]);
-    if (S > 1)
-      for (int c = 0; c < S; ++c)
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_map_shared(at, c)), "f"(v) : "memory");
-    else
-      part_sum[0][e] = v;
+    for (int w = 1; w < C::kSums; ++w) {
+      const float4 o = *reinterpret_cast<const float4*>(warp_sum + w * C::kElems + e);
+      v.x += o.x;
+      v.y += o.y;
+      v.z += o.z;
+      v.w += o.w;
+    }
+    const uint32_t at = smem_u32(part_sum + rank * C::kElems + e);
+    for (int c = 0; c < S; ++c)
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_map_shared(at, c)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                   : "memory");
   }
   if (S > 1) cluster_sync();
   else __syncthreads();
-  for (int e = threadIdx.x; e < kH; e += kFewThreads) {
-    float v = 0.f;
-    if (e < kRanks * kFew)
-      for (int c = 0; c < S; ++c) v += part_sum[c][e];
-    h[e] = v;
-    if (p.inner != nullptr && slot == 0 && e / kFew < p.rank && e % kFew < f.count) {
-      const int64_t row = lora_row(p.ids, f.place + e % kFew, p.rows);
-      if (row >= 0) p.inner[row * p.rank + e / kFew] = v;
+  // the inner vectors, and from them the second product's operand: warp w makes group w's; lane (g, s4) has row g and the ranks
+  // r * 32 + s4 * 8 .. + 7 of every block r
+  if (warp < NT) {
+    const int n = warp;
+    const bool mine = n * 8 + g < f.count;
+    const int32_t row = mine ? static_cast<int32_t>(lora_row(p.ids, f.place + n * 8 + g, p.rows)) : -1;
+    float v[C::kBlocks][8], most = 0.f;
+#pragma unroll
+    for (int r = 0; r < C::kBlocks; ++r)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = r * 32 + s4 * 8 + i;
+        float sum = 0.f;
+        if (j < C::kRanks)
+          for (int c = 0; c < S; ++c) sum += part_sum[c * C::kElems + j * C::kRows + n * 8 + g];
+        v[r][i] = sum;
+        most = fmaxf(most, fabsf(sum));
+        if (p.inner != nullptr && slot == 0 && row >= 0 && j < p.rank) p.inner[static_cast<int64_t>(row) * p.rank + j] = sum;
+      }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    float down, up;
+    row_scale(most, &down, &up);
+    if (s4 == 0) ups[n * 8 + g] = up;
+#pragma unroll
+    for (int r = 0; r < C::kBlocks; ++r) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f0 = v[r][2 * i] * down, f1 = v[r][2 * i + 1] * down;
+        hi[i] = Pair<T>::pack(f0, f1);
+        const float2 w = Pair<T>::unpack(hi[i]);
+        lo[i] = Pair<T>::pack(f0 - w.x, f1 - w.y);
+      }
+      frag[((n * C::kBlocks + r) * 2 + 0) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      frag[((n * C::kBlocks + r) * 2 + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
   __syncthreads();
 
-  // ---- second product ----
-  uint32_t hi[kBlocks][4], lo[kBlocks][4];
-  float down, up;
-  {
-    float v[kBlocks][8], most = 0.f;
-#pragma unroll
-    for (int r = 0; r < kBlocks; ++r)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[r][i] = h[(r * 32 + s4 * 8 + i) * kFew + g];
-        most = fmaxf(most, fabsf(v[r][i]));
-      }
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    row_scale(most, &down, &up);
-#pragma unroll
-    for (int r = 0; r < kBlocks; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f0 = v[r][2 * i] * down, f1 = v[r][2 * i + 1] * down;
-        hi[r][i] = Pair<T>::pack(f0, f1);
-        const float2 w = Pair<T>::unpack(hi[r][i]);
-        lo[r][i] = Pair<T>::pack(f0 - w.x, f1 - w.y);
-      }
-  }
-  // this lane's outputs are of the rows 2 s4 and 2 s4 + 1
-  float c[2];
-  int64_t out_row[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    c[i] = scale * __shfl_sync(0xffffffffu, up, (2 * s4 + i) * 4);
-    out_row[i] = __shfl_sync(0xffffffffu, my_row, (2 * s4 + i) * 4);
-  }
+  // ---- second product: B's rows n .. n + 7 in this lane, then group by group; the lane's outputs are of the rows 2 s4, 2 s4 + 1 ----
   for (int64_t unit = unit0 + warp; unit < unit1; unit += kFewWarps) {
-    const int64_t n = unit * kUnit + g * 8;   // rows n .. n + 7 of B
-    const bool in = n < p.d_out;
-    uint4 y0[2];
+    const int64_t col = unit * kUnit + g * 8;
+    const bool in = col < p.d_out;
+    uint4 w[C::kBlocks][8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      y0[i] = out_row[i] >= 0 && in ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + out_row[i] * p.ld_base + n)
-                                    : make_uint4(0u, 0u, 0u, 0u);
-    float d[4][4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) d[t][i] = 0.f;
-#pragma unroll
-    for (int r = 0; r < kBlocks; ++r) {
-      uint4 w[8];
+    for (int r = 0; r < C::kBlocks; ++r) {
       const int j = r * 32 + s4 * 8;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const bool take = in && j < p.rank;
-        w[i] = load16(b + (take ? (n + i) * p.rank + j : 0), take);
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const uint4 e = w[2 * t], o = w[2 * t + 1];
-        mma16816<T>(d[t], e.x, o.x, e.y, o.y, hi[r][0], hi[r][1]);
-        mma16816<T>(d[t], e.z, o.z, e.w, o.w, hi[r][2], hi[r][3]);
-        mma16816<T>(d[t], e.x, o.x, e.y, o.y, lo[r][0], lo[r][1]);
-        mma16816<T>(d[t], e.z, o.z, e.w, o.w, lo[r][2], lo[r][3]);
+        w[r][i] = load16(b + (take ? (col + i) * p.rank + j : 0), take);
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (out_row[i] < 0 || !in) continue;
-      uint32_t y[4] = {y0[i].x, y0[i].y, y0[i].z, y0[i].w};
+    for (int n = 0; n < NT; ++n) {
+      if (n >= groups) break;
+      int32_t to[2];
+      uint4 y0[2];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float2 v = Pair<T>::unpack(y[t]);
-        y[t] = Pair<T>::pack(fmaf(c[i], d[t][i], v.x), fmaf(c[i], d[t][2 + i], v.y));
+      for (int i = 0; i < 2; ++i) {
+        to[i] = __shfl_sync(0xffffffffu, my_row[n], (2 * s4 + i) * 4);
+        y0[i] = to[i] >= 0 && in ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + to[i] * p.ld_base + col)
+                                 : make_uint4(0u, 0u, 0u, 0u);
       }
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row[i] * p.ld_out + n) = make_uint4(y[0], y[1], y[2], y[3]);
+      float d[4][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[t][i] = 0.f;
+#pragma unroll
+      for (int r = 0; r < C::kBlocks; ++r) {
+        const uint4 hi = frag[((n * C::kBlocks + r) * 2 + 0) * 32 + lane], lo = frag[((n * C::kBlocks + r) * 2 + 1) * 32 + lane];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint4 e = w[r][2 * t], o = w[r][2 * t + 1];
+          mma16816<T>(d[t], e.x, o.x, e.y, o.y, hi.x, hi.y);
+          mma16816<T>(d[t], e.z, o.z, e.w, o.w, hi.z, hi.w);
+          mma16816<T>(d[t], e.x, o.x, e.y, o.y, lo.x, lo.y);
+          mma16816<T>(d[t], e.z, o.z, e.w, o.w, lo.z, lo.w);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (to[i] < 0 || !in) continue;
+        const float c = scale * ups[n * 8 + 2 * s4 + i];
+        uint32_t y[4] = {y0[i].x, y0[i].y, y0[i].z, y0[i].w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float2 v = Pair<T>::unpack(y[t]);
+          y[t] = Pair<T>::pack(fmaf(c, d[t][i], v.x), fmaf(c, d[t][2 + i], v.y));
+        }
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to[i] * p.ld_out + col) = make_uint4(y[0], y[1], y[2], y[3]);
+      }
     }
   }
+}
+
+template <typename T, int RT, int NT>
+ks_status_t launch_few(const char* where, const LoraPass& p, cudaStream_t stream) {
+  using C = FewCfg<RT, NT>;
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 0 && dev < 64 && !done[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(lora_few_kernel<T, RT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+      if (e != cudaSuccess) return cuda_status(e, where);
+      done[dev] = true;
+    }
+  }
+  const int64_t items = lora_tile_bound(p.rows, p.adapters, C::kRows);
+  const int64_t room = static_cast<int64_t>(sm_count()) * 2;
+  int s = kFewCluster;
+  while (s > 1 && p.d_in < 64 * s) s /= 2;
+  // several clusters per item while SMs are idle and the second product is still the larger part of each
+  int parts = 1;
+  while (items * s * parts * 2 <= room && p.d_out >= 2 * parts * p.d_in && p.d_out >= int64_t(kUnit) * s * parts * 2) parts *= 2;
+  if (items * s * parts > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
+  launch_programmatic_cluster(lora_few_kernel<T, RT, NT>, static_cast<unsigned>(items * s * parts), static_cast<unsigned>(s), true,
+                              kFewThreads, C::kSmem, stream, p, s, parts);
+  KSB_CHECK_LAUNCH(where);
+  return KS_SUCCESS;
+}
+
+template <typename T, int RT>
+ks_status_t launch_few_groups(const char* where, const LoraPass& p, cudaStream_t stream) {
+  // groups of 8 rows per item: as many as an adapter has on average
+  const int64_t mean = (p.rows + p.adapters - 1) / p.adapters;
+  return mean <= 8 ? launch_few<T, RT, 1>(where, p, stream)
+         : mean <= 16 ? launch_few<T, RT, 2>(where, p, stream)
+                      : launch_few<T, RT, 4>(where, p, stream);
+}
+
+template <typename T>
+ks_status_t launch_few_ranks(const char* where, const LoraPass& p, cudaStream_t stream) {
+  return p.rank <= 16   ? launch_few_groups<T, 1>(where, p, stream)
+         : p.rank <= 32 ? launch_few_groups<T, 2>(where, p, stream)
+         : p.rank <= 64 ? launch_few_groups<T, 4>(where, p, stream)
+                        : launch_few_groups<T, 8>(where, p, stream);
 }
 
 }  // namespace
 
 ks_status_t lora_few_pass(const char* where, const LoraPass& p, ks_dtype_t dtype, cudaStream_t stream) {
-  const int64_t items = lora_tile_bound(p.rows, p.adapters, kFew);
-  const int64_t room = static_cast<int64_t>(sm_count()) * 2;
-  int s = kFewCluster;
-  while (s > 1 && (p.d_in < 64 * s || items * s > 8 * room)) s /= 2;
-  // several clusters per item while SMs are idle and the second product is still the larger part of each
-  int parts = 1;
-  while (items * s * parts * 2 <= room && p.d_out >= 2 * parts * p.d_in && p.d_out >= int64_t(kUnit) * s * parts * 2) parts *= 2;
-  if (items * s * parts > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
-  const unsigned grid = static_cast<unsigned>(items * s * parts);
-#define KSB_LORA_FEW(T, RT) launch_programmatic_cluster(lora_few_kernel<T, RT>, grid, s, true, kFewThreads, 0, stream, p, s, parts)
-#define KSB_LORA_FEW_T(T)                     \
-  do {                                        \
-    if (p.rank <= 16) KSB_LORA_FEW(T, 1);     \
-    else if (p.rank <= 32) KSB_LORA_FEW(T, 2); \
-    else if (p.rank <= 64) KSB_LORA_FEW(T, 4); \
-    else KSB_LORA_FEW(T, 8);                  \
-  } while (0)
-  if (dtype == KS_DTYPE_F16) KSB_LORA_FEW_T(__half);
-  else KSB_LORA_FEW_T(__nv_bfloat16);
-#undef KSB_LORA_FEW_T
-#undef KSB_LORA_FEW
-  KSB_CHECK_LAUNCH(where);
-  return KS_SUCCESS;
+  return dtype == KS_DTYPE_F16 ? launch_few_ranks<__half>(where, p, stream) : launch_few_ranks<__nv_bfloat16>(where, p, stream);
 }
 
 }  // namespace sm100

@@ -871,9 +871,8 @@ ks_status_t lora_tile_pass(const char* where, const LoraPass& p, bool forward, k
   const int64_t tiles = lora_tile_bound(p.rows, p.adapters, kTile);
   const bool wide = p.rank > 64;
   const int64_t room = static_cast<int64_t>(sm_count()) * (wide ? 1 : 2);
-  const int64_t filled = (p.rows + kTile - 1) / kTile;
   int s = 1;
-  while (s < kMaxCluster && filled * s * 2 <= room) s *= 2;
+  while (s < kMaxCluster && tiles * s * 2 <= room) s *= 2;
   q.cluster = s;
   if (tiles * s > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
 #define KSB_LORA_TILE(T, FWD)                                                      \
