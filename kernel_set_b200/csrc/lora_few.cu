@@ -59,7 +59,7 @@ struct FewCfg {
 };
 
 template <typename T, int RT, int NT>
-__global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_kernel(const __grid_constant__ LoraPass p, int S, int parts) {
+__global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_kernel(const __grid_constant__ LoraPass p, int s_log, int parts_log) {
   using C = FewCfg<RT, NT>;
   extern __shared__ __align__(16) unsigned char few_smem[];
   float* warp_sum = reinterpret_cast<float*>(few_smem);
@@ -67,16 +67,16 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_
   uint4* frag = reinterpret_cast<uint4*>(few_smem + C::kFrag);          // [group][block][high, low][lane]
   float* ups = reinterpret_cast<float*>(few_smem + C::kUp);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, s4 = lane & 3;
-  const int rank = blockIdx.x % S;
-  const int part = (blockIdx.x / S) % parts;
-  const int64_t item = blockIdx.x / (S * parts);
+  const int S = 1 << s_log;                                             // CTAs of a cluster; 1 << parts_log clusters per item
+  const int rank = blockIdx.x & (S - 1);
+  const int slot = blockIdx.x & ((1 << (s_log + parts_log)) - 1);       // of the item's CTAs
+  const int64_t item = blockIdx.x >> (s_log + parts_log);
   if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (waited for before the first remote store)
   grid_dependency_wait();
   const TilePlace f = find_tile<C::kRows>(p.offsets, p.adapters, p.rows, item);
   // outputs of this CTA, in units
   const int64_t units = (p.d_out + kUnit - 1) / kUnit;
-  const int slot = part * S + rank;
-  const int64_t unit0 = units * slot / (S * parts), unit1 = units * (slot + 1) / (S * parts);
+  const int64_t unit0 = units * slot >> (s_log + parts_log), unit1 = units * (slot + 1) >> (s_log + parts_log);
   if (f.adapter < 0 || f.adapter >= p.adapters) {
     if (f.adapter == p.adapters && p.out != p.base) {
       const int64_t end = unit1 * kUnit < p.d_out ? unit1 * kUnit : p.d_out;
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_
 
   // ---- first product: blocks of 32 k, warp by warp ----
   const int64_t blocks = (p.d_in + 31) / 32;
-  const int64_t block0 = blocks * rank / S, block1 = blocks * (rank + 1) / S;
+  const int64_t block0 = blocks * rank >> s_log, block1 = blocks * (rank + 1) >> s_log;
   float acc[RT][NT][4];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
@@ -191,25 +191,46 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_
   }
   if (S > 1) cluster_sync();
   else __syncthreads();
-  // the inner vectors, and from them the second product's operand: warp w makes group w's; lane (g, s4) has row g and the ranks
-  // r * 32 + s4 * 8 .. + 7 of every block r
-  if (warp < NT) {
+  // the inner vectors, added up by all threads over the first CTA's sums
+  for (int e = threadIdx.x * 4; e < C::kElems; e += kFewThreads * 4) {
+    float4 part[kFewCluster];
+#pragma unroll
+    for (int c = 0; c < kFewCluster; ++c)
+      if (c < S) part[c] = *reinterpret_cast<const float4*>(part_sum + c * C::kElems + e);
+    float4 v = part[0];
+#pragma unroll
+    for (int c = 1; c < kFewCluster; ++c)
+      if (c < S) {
+        v.x += part[c].x;
+        v.y += part[c].y;
+        v.z += part[c].z;
+        v.w += part[c].w;
+      }
+    *reinterpret_cast<float4*>(part_sum + e) = v;
+  }
+  __syncthreads();
+  // and from them the second product's operand: warp n makes group n's; lane (g, s4) has row g and the ranks r * 32 + s4 * 8 .. + 7
+  // of every block r
+  if (warp < groups) {
     const int n = warp;
-    const bool mine = n * 8 + g < f.count;
-    const int32_t row = mine ? static_cast<int32_t>(lora_row(p.ids, f.place + n * 8 + g, p.rows)) : -1;
+    const int32_t row = n * 8 + g < f.count ? static_cast<int32_t>(lora_row(p.ids, f.place + n * 8 + g, p.rows)) : -1;
     float v[C::kBlocks][8], most = 0.f;
 #pragma unroll
     for (int r = 0; r < C::kBlocks; ++r)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int j = r * 32 + s4 * 8 + i;
-        float sum = 0.f;
-        if (j < C::kRanks)
-          for (int c = 0; c < S; ++c) sum += part_sum[c * C::kElems + j * C::kRows + n * 8 + g];
-        v[r][i] = sum;
-        most = fmaxf(most, fabsf(sum));
-        if (p.inner != nullptr && slot == 0 && row >= 0 && j < p.rank) p.inner[static_cast<int64_t>(row) * p.rank + j] = sum;
+        v[r][i] = j < C::kRanks ? part_sum[j * C::kRows + n * 8 + g] : 0.f;
+        most = fmaxf(most, fabsf(v[r][i]));
       }
+    if (p.inner != nullptr && slot == 0 && row >= 0)
+#pragma unroll
+      for (int r = 0; r < C::kBlocks; ++r)
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)
+          if (r * 32 + s4 * 8 + i < p.rank)
+            *reinterpret_cast<float4*>(p.inner + static_cast<int64_t>(row) * p.rank + r * 32 + s4 * 8 + i) =
+                make_float4(v[r][i], v[r][i + 1], v[r][i + 2], v[r][i + 3]);
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     float down, up;
@@ -245,17 +266,18 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_
         w[r][i] = load16(b + (take ? (col + i) * p.rank + j : 0), take);
       }
     }
+    uint4 y0[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int32_t to = __shfl_sync(0xffffffffu, my_row[n], (2 * s4 + i) * 4);
+        y0[n][i] = to >= 0 && in ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + to * p.ld_base + col)
+                                 : make_uint4(0u, 0u, 0u, 0u);
+      }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       if (n >= groups) break;
-      int32_t to[2];
-      uint4 y0[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        to[i] = __shfl_sync(0xffffffffu, my_row[n], (2 * s4 + i) * 4);
-        y0[i] = to[i] >= 0 && in ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + to[i] * p.ld_base + col)
-                                 : make_uint4(0u, 0u, 0u, 0u);
-      }
       float d[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -275,15 +297,16 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (to[i] < 0 || !in) continue;
+        const int32_t to = __shfl_sync(0xffffffffu, my_row[n], (2 * s4 + i) * 4);
+        if (to < 0 || !in) continue;
         const float c = scale * ups[n * 8 + 2 * s4 + i];
-        uint32_t y[4] = {y0[i].x, y0[i].y, y0[i].z, y0[i].w};
+        uint32_t y[4] = {y0[n][i].x, y0[n][i].y, y0[n][i].z, y0[n][i].w};
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const float2 v = Pair<T>::unpack(y[t]);
           y[t] = Pair<T>::pack(fmaf(c, d[t][i], v.x), fmaf(c, d[t][2 + i], v.y));
         }
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to[i] * p.ld_out + col) = make_uint4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to * p.ld_out + col) = make_uint4(y[0], y[1], y[2], y[3]);
       }
     }
   }
@@ -306,14 +329,15 @@ ks_status_t launch_few(const char* where, const LoraPass& p, cudaStream_t stream
   }
   const int64_t items = lora_tile_bound(p.rows, p.adapters, C::kRows);
   const int64_t room = static_cast<int64_t>(sm_count()) * 2;
-  int s = kFewCluster;
-  while (s > 1 && p.d_in < 64 * s) s /= 2;
+  int s = 3;   // logarithms
+  static_assert(kFewCluster == 8, "");
+  while (s > 0 && p.d_in < 64 << s) --s;
   // several clusters per item while SMs are idle and the second product is still the larger part of each
-  int parts = 1;
-  while (items * s * parts * 2 <= room && p.d_out >= 2 * parts * p.d_in && p.d_out >= int64_t(kUnit) * s * parts * 2) parts *= 2;
-  if (items * s * parts > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
-  launch_programmatic_cluster(lora_few_kernel<T, RT, NT>, static_cast<unsigned>(items * s * parts), static_cast<unsigned>(s), true,
-                              kFewThreads, C::kSmem, stream, p, s, parts);
+  int parts = 0;
+  while (items << (s + parts + 1) <= room && p.d_out >= p.d_in << (parts + 1) && p.d_out >= int64_t(kUnit) << (s + parts + 1)) ++parts;
+  if (items << (s + parts) > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
+  launch_programmatic_cluster(lora_few_kernel<T, RT, NT>, static_cast<unsigned>(items << (s + parts)), 1u << s, true, kFewThreads,
+                              C::kSmem, stream, p, s, parts);
   KSB_CHECK_LAUNCH(where);
   return KS_SUCCESS;
 }

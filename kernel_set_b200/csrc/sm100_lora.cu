@@ -119,25 +119,30 @@ struct TileParams {
   unsigned int* fault_word;
   uint32_t idesc1, idesc2;
   int rank16;       // rank rounded up to 16
-  int cluster;
+  int cluster_log;  // CTAs of a cluster: 1 << cluster_log
+  int in_chunks, out_chunks;
 };
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // CTA `rank` of S adds up its part of the cluster's sums, in rank order, and writes the totals back to all of them, where only it has
-// read. A thread has eight 16-byte loads from other SMs in flight.
+// read. Piece e is the 16 bytes of row e % rows and four ranks. A thread has eight loads from other SMs in flight.
 template <int S, int THREADS>
-__device__ __forceinline__ void reduce_scatter(uint32_t exchange, int pieces, int rank) {
+__device__ __forceinline__ void reduce_scatter(uint32_t exchange, int pieces, int quarters, int rank) {
   constexpr int kAtOnce = kMaxCluster / S;
   const int end = pieces / S * (rank + 1);
   for (int e0 = pieces / S * rank + threadIdx.x; e0 < end; e0 += kAtOnce * THREADS) {
     float4 part[kAtOnce][S];
+    uint32_t at[kAtOnce];
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u)
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int e = e0 + u * THREADS, j = (e >> 5) / quarters, row = e - j * quarters * 32;
+      at[u] = exchange + (j * kTile + row) * 16;
 #pragma unroll
       for (int c = 0; c < S; ++c)
-        if (e0 + u * THREADS < end) part[u][c] = ld_shared_cluster_f4(cluster_map_shared(exchange + (e0 + u * THREADS) * 16, c));
+        if (e < end) part[u][c] = ld_shared_cluster_f4(cluster_map_shared(at[u], c));
+    }
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u) {
       if (e0 + u * THREADS >= end) continue;
@@ -150,7 +155,7 @@ __device__ __forceinline__ void reduce_scatter(uint32_t exchange, int pieces, in
         sum.w += part[u][c].w;
       }
 #pragma unroll
-      for (int c = 0; c < S; ++c) st_shared_cluster_f4(cluster_map_shared(exchange + (e0 + u * THREADS) * 16, c), sum);
+      for (int c = 0; c < S; ++c) st_shared_cluster_f4(cluster_map_shared(at[u], c), sum);
     }
   }
 }
@@ -178,8 +183,8 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
   volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(bar_mem + C::kBars);   // tmem address, abort, tile
   const WaitCtx wctx{smem_u32(const_cast<uint32_t*>(words) + 1), q.fault_word};
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int S = q.cluster;
-  const uint32_t rank = blockIdx.x % S;
+  const int S = 1 << q.cluster_log;
+  const uint32_t rank = blockIdx.x & (S - 1);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
     tmem_relinquish();
   }
   if (warp == 0) {
-    const TilePlace f = find_tile<kTile>(p.offsets, p.adapters, p.rows, blockIdx.x / S);
+    const TilePlace f = find_tile<kTile>(p.offsets, p.adapters, p.rows, blockIdx.x >> q.cluster_log);
     if (lane == 0) {
       words[2] = static_cast<uint32_t>(f.adapter);
       words[3] = static_cast<uint32_t>(f.count);
@@ -228,11 +233,10 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
   const int64_t place = words[4];
 
   // this CTA's 64-column chunks of the inputs and of the outputs
-  const int in_chunks = static_cast<int>((p.d_in + kChunk - 1) / kChunk), out_chunks = static_cast<int>((p.d_out + kChunk - 1) / kChunk);
-  const int in0 = static_cast<int>(static_cast<int64_t>(in_chunks) * rank / S);
-  const int n1 = static_cast<int>(static_cast<int64_t>(in_chunks) * (rank + 1) / S) - in0;
-  const int out0 = static_cast<int>(static_cast<int64_t>(out_chunks) * rank / S);
-  const int n2 = static_cast<int>(static_cast<int64_t>(out_chunks) * (rank + 1) / S) - out0;
+  const auto share = [&](int chunks, uint32_t r) { return static_cast<int>((static_cast<uint32_t>(chunks) * r) >> q.cluster_log); };
+  const int in0 = share(q.in_chunks, rank), n1 = share(q.in_chunks, rank + 1) - in0;
+  const int out0 = share(q.out_chunks, rank), n2 = share(q.out_chunks, rank + 1) - out0;
+  const int quarters = (count + 31) / 32;   // of the tile that hold rows
 
   if (adapter == p.adapters) {
     // rows without an adapter: y = y0
@@ -293,8 +297,10 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         const bool in_width = col + c8 * 8 < width;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const bool take = in_width && (have >> i & 1u);
-          cp_async16(dst + r0 * 128 + ((c8 ^ (r0 & 7)) << 4) + i * 2048, take ? src[i] : p.in, take);
+          // (places without a row are cleared once; what the epilogue leaves there is zero again)
+          const bool row = have >> i & 1u;
+          if (row || it < C::kStages)
+            cp_async16(dst + r0 * 128 + ((c8 ^ (r0 & 7)) << 4) + i * 2048, row && in_width ? src[i] : p.in, row && in_width);
           src[i] += kChunk;
         }
         const uint32_t wdst = dst + kRowsBytes;
@@ -367,13 +373,14 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
       const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter) << 21);
       const float s = __ldg(p.scales + adapter);
       const int blocks = q.rank16 / 16;
+      const bool used = quarter < quarters;   // (the quarters without rows only keep step)
       if (!joined) cluster_wait();
       joined = true;
       bool ok = n1 == 0 || mbar_wait_long(wctx, bar_sums, 0, 0x37);
       tc_fence_after_sync();
       if (ok && S > 1) {
         // ranks 4 j .. of row r at exchange + (j * 128 + r) * 16
-        for (int b = half; b < blocks; b += 2) {
+        for (int b = used ? half : blocks; b < blocks; b += 2) {
           uint32_t x[16];
           if (n1 > 0) {
             tmem_ld(lanes + b * 16, x);
@@ -390,10 +397,10 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         if (lane < S) mbar_arrive_cluster(bar_parts, lane);
         ok = mbar_wait_cluster(wctx, bar_parts, 0, 0x38);
         if (ok) {
-          const int pieces = q.rank16 / 4 * kTile;
-          if (S == 2) reduce_scatter<2, C::kEpiWarps * 32>(exchange, pieces, rank);
-          else if (S == 4) reduce_scatter<4, C::kEpiWarps * 32>(exchange, pieces, rank);
-          else reduce_scatter<8, C::kEpiWarps * 32>(exchange, pieces, rank);
+          const int pieces = q.rank16 / 4 * quarters * 32;
+          if (S == 2) reduce_scatter<2, C::kEpiWarps * 32>(exchange, pieces, quarters, rank);
+          else if (S == 4) reduce_scatter<4, C::kEpiWarps * 32>(exchange, pieces, quarters, rank);
+          else reduce_scatter<8, C::kEpiWarps * 32>(exchange, pieces, quarters, rank);
           __syncwarp();
           if (lane < S) mbar_arrive_cluster(bar_total, lane);
           ok = mbar_wait_cluster(wctx, bar_total, 0, 0x3b);
@@ -417,7 +424,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         };
         const int32_t row = row_of[r];
         float most = 0.f, down, up;
-        for (int b = 0; b < blocks; ++b) {
+        for (int b = used ? 0 : blocks; b < blocks; ++b) {
           uint32_t x[16];
           sums_of(b, x);
 #pragma unroll
@@ -428,7 +435,12 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         float* inner = p.inner != nullptr && rank == 0 && row >= 0 ? p.inner + static_cast<int64_t>(row) * p.rank : nullptr;
         for (int b = half; b < blocks; b += 2) {
           uint32_t x[16], hi[8], lo[8];
-          sums_of(b, x);
+          if (used) {
+            sums_of(b, x);
+          } else {   // (rows of zeros, whatever tensor memory held)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = 0u;
+          }
           if (inner != nullptr) {
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
@@ -479,45 +491,46 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
 #pragma unroll 1
         for (int j = 0; j < n2; ++j) {
           const int it = n1 + j, st = it % C::kStages, b = j & 1;
-          if (!mbar_wait(wctx, out_full(b), (j >> 1) & 1, 0x39)) break;
-          if (!mbar_wait(wctx, full(st), (it / C::kStages) & 1, 0x3a)) break;
-          tc_fence_after_sync();
           const uint32_t tile = ring + st * C::kStageBytes;
+          if (!mbar_wait(wctx, full(st), (it / C::kStages) & 1, 0x3a)) break;
+          uint4 y[4];
+          if (used) {
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            uint32_t d[16];
-            tmem_ld(lanes + C::kOut + b * kChunk + half * 32 + part * 16, d);
-            tmem_wait_ld(d);
-            if (part == 1) {
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(out_free(b));
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t at = tile + r * 128 + (((half * 4 + part * 2 + i) ^ (r & 7)) << 4);
-              const uint4 y0 = ld_shared_v4(at);
-              uint32_t y[4] = {y0.x, y0.y, y0.z, y0.w};
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const float2 f = Pair<T>::unpack(y[w]);
-                y[w] = Pair<T>::pack(fmaf(c, __uint_as_float(d[i * 8 + w * 2]), f.x),
-                                     fmaf(c, __uint_as_float(d[i * 8 + w * 2 + 1]), f.y));
-              }
-              st_shared_v4(at, y[0], y[1], y[2], y[3]);
-            }
+            for (int i = 0; i < 4; ++i) y[i] = ld_shared_v4(tile + r * 128 + (((half * 4 + i) ^ (r & 7)) << 4));
           }
-          asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");   // (both halves of the quarter's rows are there)
-          const bool in_width = static_cast<int64_t>(out0 + j) * kChunk + piece * 8 < p.d_out;
+          if (!mbar_wait(wctx, out_full(b), (j >> 1) & 1, 0x39)) break;
+          tc_fence_after_sync();
+          if (used) {
+            uint32_t d[32];
+            tmem_ld(lanes + C::kOut + b * kChunk + half * 32, d);
+            tmem_wait_ld(d);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rr = out_row + i * 4;
-            const uint4 y = ld_shared_v4(tile + rr * 128 + ((piece ^ (rr & 7)) << 4));
-            if (in_width && (have >> i & 1u)) *reinterpret_cast<uint4*>(dst[i]) = y;
-            dst[i] += kChunk;
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[4] = {y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 f = Pair<T>::unpack(w[k]);
+                w[k] = Pair<T>::pack(fmaf(c, __uint_as_float(d[i * 8 + k * 2]), f.x),
+                                     fmaf(c, __uint_as_float(d[i * 8 + k * 2 + 1]), f.y));
+              }
+              st_shared_v4(tile + r * 128 + (((half * 4 + i) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+            }
+            tc_fence_before_sync();
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");   // (both halves of the quarter's rows are there)
+            const bool in_width = static_cast<int64_t>(out0 + j) * kChunk + piece * 8 < p.d_out;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = ld_shared_v4(tile + (out_row + i * 4) * 128 + ((piece ^ ((out_row + i * 4) & 7)) << 4));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (in_width && (have >> i & 1u)) *reinterpret_cast<uint4*>(dst[i]) = y[i];
+              dst[i] += kChunk;
+            }
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(free2(st));
+          if (lane == 0) {
+            mbar_arrive(out_free(b));
+            mbar_arrive(free2(st));
+          }
         }
       }
     }
@@ -549,7 +562,7 @@ ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, c
       done[dev] = true;
     }
   }
-  launch_programmatic_cluster(lora_tile_kernel<T, RC, FWD>, static_cast<unsigned>(tiles * q.cluster), static_cast<unsigned>(q.cluster),
+  launch_programmatic_cluster(lora_tile_kernel<T, RC, FWD>, static_cast<unsigned>(tiles << q.cluster_log), 1u << q.cluster_log,
                               true, C::kThreads, C::kSmem, stream, q);
   KSB_CHECK_LAUNCH(where);
   return KS_SUCCESS;
@@ -591,7 +604,7 @@ struct GradParams {
   LoraWeightGrad p;
   unsigned int* fault_word;
   uint32_t idesc;
-  int rank16, cluster;
+  int rank16, cluster_log;   // CTAs of a cluster: 1 << cluster_log
   int slabs_a, slabs;     // slabs of x, of both
 };
 
@@ -610,9 +623,9 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
   volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(bar_mem + C::kBars);
   const WaitCtx wctx{smem_u32(const_cast<uint32_t*>(words) + 1), q.fault_word};
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int S = q.cluster;
-  const int rank = blockIdx.x % S;
-  const int item = blockIdx.x / S;
+  const int S = 1 << q.cluster_log;
+  const int rank = blockIdx.x & (S - 1);
+  const int item = blockIdx.x >> q.cluster_log;
   const int adapter = item / q.slabs;
   const int slab = item - adapter * q.slabs;
   const bool is_a = slab < q.slabs_a;
@@ -643,8 +656,8 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
   const int64_t begin = lora_offset(p.offsets, adapter, p.rows);
   const int64_t count = max(lora_offset(p.offsets, adapter + 1, p.rows) - begin, int64_t(0));
   const int64_t chunks = (count + 63) / 64;
-  const int64_t chunk0 = chunks * rank / S;
-  const int n = static_cast<int>(chunks * (rank + 1) / S - chunk0);
+  const int64_t chunk0 = chunks * rank >> q.cluster_log;
+  const int n = static_cast<int>((chunks * (rank + 1) >> q.cluster_log) - chunk0);
   const auto row_at = [&](int64_t chunk, int i) -> int32_t {   // row i of a chunk, -1 past the end
     const int64_t at = chunk * 64 + i;
     return at < count ? static_cast<int32_t>(lora_row(p.ids, begin + at, p.rows)) : -1;
@@ -788,7 +801,7 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
   if (S > 1) cluster_sync();
   else __syncthreads();
   // the cluster's CTAs share the slab's columns; 8 numbers that lie together in the result at a time
-  const int cols = kSlab / S;   // a multiple of 8
+  const int cols = kSlab >> q.cluster_log;   // a multiple of 8
   const int64_t factor = static_cast<int64_t>(adapter) * p.rank * width;
   const auto sum_at = [&](int j, int m, int cta) {
     return cluster_map_shared(ring + (j * kSlab + m) * 4, cta);
@@ -846,7 +859,7 @@ ks_status_t launch_grad(const char* where, const GradParams& q, int64_t items, c
       done[dev] = true;
     }
   }
-  launch_programmatic_cluster(lora_weight_grad_kernel<T, RB>, static_cast<unsigned>(items * q.cluster), static_cast<unsigned>(q.cluster),
+  launch_programmatic_cluster(lora_weight_grad_kernel<T, RB>, static_cast<unsigned>(items << q.cluster_log), 1u << q.cluster_log,
                               true, C::kThreads, C::kSmem, stream, q);
   KSB_CHECK_LAUNCH(where);
   return KS_SUCCESS;
@@ -871,10 +884,11 @@ ks_status_t lora_tile_pass(const char* where, const LoraPass& p, bool forward, k
   const int64_t tiles = lora_tile_bound(p.rows, p.adapters, kTile);
   const bool wide = p.rank > 64;
   const int64_t room = static_cast<int64_t>(sm_count()) * (wide ? 1 : 2);
-  int s = 1;
-  while (s < kMaxCluster && tiles * s * 2 <= room) s *= 2;
-  q.cluster = s;
-  if (tiles * s > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
+  // the largest cluster with which all tiles that there can be run at a time
+  while ((2 << q.cluster_log) <= kMaxCluster && tiles << (q.cluster_log + 1) <= room) ++q.cluster_log;
+  q.in_chunks = static_cast<int>((p.d_in + kChunk - 1) / kChunk);
+  q.out_chunks = static_cast<int>((p.d_out + kChunk - 1) / kChunk);
+  if (tiles << q.cluster_log > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
 #define KSB_LORA_TILE(T, FWD)                                                      \
   (p.rank <= 32   ? launch_tile<T, 0, FWD>(where, q, tiles, stream)                \
    : p.rank <= 64 ? launch_tile<T, 1, FWD>(where, q, tiles, stream)                \
@@ -901,10 +915,8 @@ ks_status_t lora_weight_grad_pass(const char* where, const LoraWeightGrad& p, ks
   const bool wide = p.rank > 64;
   const int64_t items = static_cast<int64_t>(p.adapters) * q.slabs;
   const int64_t room = static_cast<int64_t>(sm_count()) * (wide ? 1 : 2);
-  int s = 1;
-  while (s < kMaxCluster && items * s * 2 <= room && p.rows > 64 * s) s *= 2;
-  q.cluster = s;
-  if (items * s > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
+  while ((2 << q.cluster_log) <= kMaxCluster && items << (q.cluster_log + 1) <= room && p.rows > 64 << q.cluster_log) ++q.cluster_log;
+  if (items << q.cluster_log > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
   if (dtype == KS_DTYPE_F16)
     return wide ? launch_grad<__half, 2>(where, q, items, stream) : launch_grad<__half, 1>(where, q, items, stream);
   return wide ? launch_grad<__nv_bfloat16, 2>(where, q, items, stream) : launch_grad<__nv_bfloat16, 1>(where, q, items, stream);
