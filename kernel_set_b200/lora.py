@@ -14,12 +14,13 @@ operator of this kind."""
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional
 
 import torch
 
 from ._lib import by_address as lib, check
-from ._tensor import TensorLike, default_stream, dtype_to_ks, f32_ptr, i32_ptr, on_device_of, ptr, same_dtype, stream_ptr
+from ._tensor import TensorLike, default_stream, dtype_to_ks, i32_ptr, on_device_of, ptr, stream_ptr
 
 
 def plan(adapter_ids: torch.Tensor, num_adapters: int, sorted_ids: Optional[torch.Tensor] = None,
@@ -47,37 +48,47 @@ def _sizes(**pairs) -> None:
             raise ValueError(f"{what}: {got} where {want} is expected")
 
 
-def _rows(t: torch.Tensor, name: str, rows: int, cols: int):
-    """Address and leading dimension of a matrix whose rows are contiguous."""
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor (got device {t.device}); kernel_set operates on device memory")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise ValueError(f"{name} must be [{rows}, {cols}]; got {list(t.shape)}")
-    if cols > 1 and t.stride(1) != 1:
-        raise ValueError(f"the rows of {name} must be contiguous")
-    ld = t.stride(0) if rows > 1 else cols
-    if ld < cols:
-        raise ValueError(f"the rows of {name} overlap")
-    return t.data_ptr(), ld
+def _ld(t: torch.Tensor, rows: int, cols: int) -> int:
+    """Elements from a row of ``t`` to the next; -1 where its rows are not contiguous or overlap."""
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1:
+        return -1
+    return cols if rows <= 1 else (ld if ld >= cols else -1)
 
 
-def _problem(x, a, b, scales, sorted_ids, offsets):
-    if a.dim() != 3 or b.dim() != 3 or x.dim() != 2:
-        raise ValueError("x must be [tokens, K], a [adapters, rank, K], b [adapters, N, rank]")
-    adapters, rank, k = a.shape
-    n = b.shape[1]
-    tokens = x.shape[0]
-    _sizes(b=(tuple(b.shape), (adapters, n, rank)), scales=(scales.numel(), adapters))
+def _refuse(rows: dict, flat: dict, sorted_ids, offsets, adapters: int) -> None:
+    """The message for a call that the wrappers' quick test does not let through: ``rows`` are matrices with contiguous
+    rows (tensor, shape, dtype), ``flat`` contiguous tensors."""
+    for name, (t, shape, dtype) in {**rows, **flat}.items():
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must be {list(shape)}; got {list(t.shape)}")
+        if t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}; got {t.dtype}")
     if offsets.numel() < adapters + 1:
         raise ValueError(f"offsets: {offsets.numel()} entries where at least {adapters + 1} are expected")
-    if sorted_ids is not None:
-        _sizes(sorted_ids=(sorted_ids.numel(), tokens))
-    if scales.dtype != torch.float32:
-        raise ValueError(f"scales must be float32; got {scales.dtype}")
-    for name, t in (("sorted_ids", sorted_ids), ("offsets", offsets)):
-        if t is not None and t.dtype != torch.int32:
-            raise ValueError(f"{name} must be int32; got {t.dtype}")
-    return tokens, adapters, rank, k, n
+    if offsets.dtype != torch.int32:
+        raise ValueError(f"offsets must be int32; got {offsets.dtype}")
+    for name, (t, shape, dtype) in rows.items():
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (got device {t.device}); kernel_set operates on device memory")
+        if _ld(t, *shape) < 0:
+            raise ValueError(f"the rows of {name} must be contiguous and apart")
+    for name, (t, shape, dtype) in flat.items():
+        ptr(t, name=name)
+    ptr(offsets, name="offsets")
+    raise AssertionError("unreachable")
+
+
+def _dims(x: torch.Tensor, b: torch.Tensor):
+    if x.dim() != 2 or b.dim() != 3:
+        raise ValueError("x must be [tokens, K], a [adapters, rank, K], b [adapters, N, rank]")
+    return (*x.shape, *b.shape)
+
+
+def _plan_ok(sorted_ids, offsets, tokens: int, adapters: int) -> bool:
+    return (offsets.dtype is torch.int32 and offsets.is_cuda and offsets.is_contiguous() and offsets.numel() > adapters
+            and (sorted_ids is None or (sorted_ids.dtype is torch.int32 and sorted_ids.is_cuda and sorted_ids.is_contiguous()
+                                        and sorted_ids.numel() == tokens)))
 
 
 def apply(out: torch.Tensor, base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor,
@@ -88,23 +99,31 @@ def apply(out: torch.Tensor, base: torch.Tensor, x: torch.Tensor, a: torch.Tenso
     ``x [tokens, K]``, ``base`` and ``out [tokens, N]`` (``out`` may be ``base``; rows contiguous, any distance apart,
     so a slice of a fused projection's columns will do), ``a [adapters, rank, K]``, ``b [adapters, N, rank]``, all f16 or bf16;
     ``scales [adapters]`` fp32; ``h [tokens, rank]`` fp32 receives ``A x`` for :func:`backward`."""
-    tokens, adapters, rank, k, n = _problem(x, a, b, scales, sorted_ids, offsets)
-    same_dtype(x, out=out, base=base, a=a, b=b)
-    out_ptr, ld_out = _rows(out, "out", tokens, n)
-    base_ptr, ld_base = _rows(base, "base", tokens, n)
-    x_ptr, ld_x = _rows(x, "x", tokens, k)
-    if h is not None:
-        if h.dtype != torch.float32:
-            raise ValueError(f"h must be float32; got {h.dtype}")
-        _sizes(h=(tuple(h.shape), (tokens, rank)))
+    tokens, k, adapters, n, rank = _dims(x, b)
+    dt = x.dtype
+    # one quick test of everything: the smallest calls are bound by the host's path
+    if not (out.shape == base.shape == (tokens, n) and a.shape == (adapters, rank, k) and scales.shape == (adapters,)
+            and out.dtype is base.dtype is a.dtype is b.dtype is dt and scales.dtype is torch.float32
+            and out.is_cuda and base.is_cuda and x.is_cuda and a.is_cuda and b.is_cuda and scales.is_cuda
+            and (ld_out := _ld(out, tokens, n)) >= 0 and (ld_base := _ld(base, tokens, n)) >= 0 and (ld_x := _ld(x, tokens, k)) >= 0
+            and a.is_contiguous() and b.is_contiguous() and scales.is_contiguous() and _plan_ok(sorted_ids, offsets, tokens, adapters)
+            and (h is None or (h.shape == (tokens, rank) and h.dtype is torch.float32 and h.is_cuda and h.is_contiguous()))):
+        flat = {"a": (a, (adapters, rank, k), dt), "b": (b, (adapters, n, rank), dt), "scales": (scales, (adapters,), torch.float32)}
+        if sorted_ids is not None:
+            flat["sorted_ids"] = (sorted_ids, (tokens,), torch.int32)
+        if h is not None:
+            flat["h"] = (h, (tokens, rank), torch.float32)
+        _refuse({"out": (out, (tokens, n), dt), "base": (base, (tokens, n), dt), "x": (x, (tokens, k), dt)}, flat, sorted_ids, offsets,
+                adapters)
     with on_device_of(x):
-        check(lib.ks_lora_apply(out_ptr, ld_out, base_ptr, ld_base, f32_ptr(h, name="h"), x_ptr, ld_x, ptr(a, name="a"),
-                                ptr(b, name="b"), f32_ptr(scales, name="scales"), i32_ptr(sorted_ids, name="sorted_ids"),
-                                i32_ptr(offsets, name="offsets"), tokens, adapters, rank, k, n, dtype_to_ks(x.dtype),
-                                default_stream(stream, x)), "ks_lora_apply")
+        check(lib.ks_lora_apply(out.data_ptr(), ld_out, base.data_ptr(), ld_base, None if h is None else h.data_ptr(), x.data_ptr(), ld_x,
+                                a.data_ptr(), b.data_ptr(), scales.data_ptr(), None if sorted_ids is None else sorted_ids.data_ptr(),
+                                offsets.data_ptr(), tokens, adapters, rank, k, n, dtype_to_ks(dt), default_stream(stream, x)),
+              "ks_lora_apply")
     return out
 
 
+@functools.lru_cache(maxsize=256)
 def backward_workspace(tokens: int, adapters: int, rank: int, k: int, n: int) -> int:
     """Bytes of workspace that :func:`backward` needs for these sizes."""
     size = ctypes.c_size_t()
@@ -122,25 +141,32 @@ def backward(d_x: torch.Tensor, d_a: torch.Tensor, d_b: torch.Tensor, d_x_base: 
     adapter's rows, zeros for an adapter without rows. ``h`` is what the forward pass kept. ``d_out`` is the gradient of
     ``base`` as it is. Types and shapes as in :func:`apply`; ``workspace``: uint8, allocated if not given.
     Returns ``(d_x, d_a, d_b)``."""
-    tokens, adapters, rank, k, n = _problem(x, a, b, scales, sorted_ids, offsets)
-    same_dtype(x, d_x=d_x, d_a=d_a, d_b=d_b, d_x_base=d_x_base, d_out=d_out, a=a, b=b)
-    _sizes(d_a=(tuple(d_a.shape), tuple(a.shape)), d_b=(tuple(d_b.shape), tuple(b.shape)),
-           h=(tuple(h.shape), (tokens, rank)))
-    if h.dtype != torch.float32:
-        raise ValueError(f"h must be float32; got {h.dtype}")
-    d_x_ptr, ld_d_x = _rows(d_x, "d_x", tokens, k)
-    d_x_base_ptr, ld_d_x_base = _rows(d_x_base, "d_x_base", tokens, k)
-    d_out_ptr, ld_d_out = _rows(d_out, "d_out", tokens, n)
-    x_ptr, ld_x = _rows(x, "x", tokens, k)
+    tokens, k, adapters, n, rank = _dims(x, b)
+    dt = x.dtype
+    if not (d_x.shape == d_x_base.shape == (tokens, k) and d_out.shape == (tokens, n) and a.shape == d_a.shape == (adapters, rank, k)
+            and d_b.shape == (adapters, n, rank) and h.shape == (tokens, rank) and scales.shape == (adapters,)
+            and d_x.dtype is d_x_base.dtype is d_out.dtype is a.dtype is d_a.dtype is b.dtype is d_b.dtype is dt
+            and h.dtype is scales.dtype is torch.float32
+            and all(t.is_cuda for t in (d_x, d_x_base, d_out, x)) and all(t.is_cuda and t.is_contiguous() for t in (a, d_a, b, d_b, h, scales))
+            and (ld_d_x := _ld(d_x, tokens, k)) >= 0 and (ld_d_x_base := _ld(d_x_base, tokens, k)) >= 0
+            and (ld_d_out := _ld(d_out, tokens, n)) >= 0 and (ld_x := _ld(x, tokens, k)) >= 0
+            and _plan_ok(sorted_ids, offsets, tokens, adapters)):
+        flat = {"a": (a, (adapters, rank, k), dt), "d_a": (d_a, (adapters, rank, k), dt), "b": (b, (adapters, n, rank), dt),
+                "d_b": (d_b, (adapters, n, rank), dt), "h": (h, (tokens, rank), torch.float32),
+                "scales": (scales, (adapters,), torch.float32)}
+        if sorted_ids is not None:
+            flat["sorted_ids"] = (sorted_ids, (tokens,), torch.int32)
+        _refuse({"d_x": (d_x, (tokens, k), dt), "d_x_base": (d_x_base, (tokens, k), dt), "d_out": (d_out, (tokens, n), dt),
+                 "x": (x, (tokens, k), dt)}, flat, sorted_ids, offsets, adapters)
     if workspace is None:
         workspace = torch.empty(backward_workspace(tokens, adapters, rank, k, n), dtype=torch.uint8, device=x.device)
         if stream is not None:   # it goes back to its pool when this returns
             workspace.record_stream(torch.cuda.ExternalStream(stream_ptr(stream), device=x.device))
     with on_device_of(x):
-        check(lib.ks_lora_backward(d_x_ptr, ld_d_x, ptr(d_a, name="d_a"), ptr(d_b, name="d_b"), d_x_base_ptr, ld_d_x_base,
-                                   d_out_ptr, ld_d_out, x_ptr, ld_x, f32_ptr(h, name="h"), ptr(a, name="a"), ptr(b, name="b"),
-                                   f32_ptr(scales, name="scales"), i32_ptr(sorted_ids, name="sorted_ids"),
-                                   i32_ptr(offsets, name="offsets"), tokens, adapters, rank, k, n,
-                                   ptr(workspace, name="workspace"), workspace.numel() * workspace.element_size(),
-                                   dtype_to_ks(x.dtype), default_stream(stream, x)), "ks_lora_backward")
+        check(lib.ks_lora_backward(d_x.data_ptr(), ld_d_x, d_a.data_ptr(), d_b.data_ptr(), d_x_base.data_ptr(), ld_d_x_base,
+                                   d_out.data_ptr(), ld_d_out, x.data_ptr(), ld_x, h.data_ptr(), a.data_ptr(), b.data_ptr(),
+                                   scales.data_ptr(), None if sorted_ids is None else sorted_ids.data_ptr(), offsets.data_ptr(), tokens,
+                                   adapters, rank, k, n, ptr(workspace, name="workspace"),
+                                   workspace.numel() * workspace.element_size(), dtype_to_ks(dt), default_stream(stream, x)),
+              "ks_lora_backward")
     return d_x, d_a, d_b
