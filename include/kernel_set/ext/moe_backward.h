@@ -39,7 +39,7 @@ KS_API ks_status_t ks_moe_gate_softmax_topk_backward(
  *   d_input [num_tokens, hidden], d_permuted [num_tokens*top_k, hidden], f32 / f16 / bf16
  *   sorted_token_ids [num_tokens*top_k] int32; a pair may occur once, rows with
  *   an id out of range are not read.
- * From 4096 pairs on, the inverse permutation lives in the stream's scratch, which
+ * In all but small calls the inverse permutation lives in the stream's scratch, which
  * this call shares with ks_moe_unpermute (the same rules under stream capture).
  */
 KS_API ks_status_t ks_moe_permute_backward(void* d_input,

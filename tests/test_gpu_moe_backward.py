@@ -72,6 +72,17 @@ def test_permute_backward(ks, cuda, tokens, experts, top_k, hidden, dropped, dty
     check("d_input", got, want, half_step(dtype) * (want.abs() + top_k * ULP * mag) + top_k * ULP * mag)
 
 
+# above 4096 pairs: slots in several groups, rows of several segments, whole and single elements
+MANY = [(200, 64, 33, 264, 0.1, BF), (150, 64, 40, 131, 0.1, HF), (700, 16, 9, 1032, 0.0, F32), (520, 32, 12, 130, 0.2, BF),
+        (513, 64, 8, 7168, 0.125, BF), (1400, 8, 3, 8200, 0.1, HF), (4200, 8, 1, 4104, 0.0, F32), (2100, 16, 2, 24, 0.9, F32),
+        (600, 8, 8, 1024, 1.0, BF)]
+
+
+@pytest.mark.parametrize("tokens,experts,top_k,hidden,dropped,dtype", MANY)
+def test_permute_backward_many_pairs(ks, cuda, tokens, experts, top_k, hidden, dropped, dtype):
+    test_permute_backward(ks, cuda, tokens, experts, top_k, hidden, dropped, dtype)
+
+
 @pytest.mark.parametrize("tokens", [50, 3000])
 def test_unaligned_rows(ks, cuda, tokens):
     """Buffers that begin off a 16-byte boundary."""
