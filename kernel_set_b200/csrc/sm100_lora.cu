@@ -576,9 +576,10 @@ ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, c
 // adapter and splits its rows; the parts are added up over distributed shared memory in rank order. Rows are contracted, so both operands
 // are stored with the contracted index outside (MN-major), as they lie in memory; a vector is split into two 16-bit
 // numbers, two MMAs. In f16 the vectors are scaled by a power of two per adapter, from the maxima that the pass before left.
-//   warps 0-3   split vectors (registers, a stage ahead -> shared memory), at the end the sums and the result
-//   warps 4-7   copies of 64 rows x 512 bytes by cp.async
-//   warp 8      tcgen05.mma: per stage 2 (128-column halves) x 4 (16 rows each) x 2 (parts), N = rank
+//   warps 0-7   split vectors (registers, two stages ahead -> shared memory, four warps a stage), at the end the sums
+//   warps 8-11  copies of 64 rows x 512 bytes: one TMA load per 128 bytes of width where the rows lie together (a sequence), cp.async where
+//               they do not (TMA gathers of four rows: 322 us against 196 for 16384 rows of 3 adapters, rank 16: a copy of 512 bytes takes 40 clocks)
+//   warp 12     tcgen05.mma: per stage 2 (128-column halves) x 4 (16 rows each) x 2 (parts), N = rank
 // Bound by memory: every element of x and dout is read once; the vectors are read again from L2 per slab (half the bytes of
 // a slab's rows at rank 64, which is why a slab is as wide as tensor memory and the ring allow two CTAs per SM).
 constexpr int kSlab = 256;
@@ -586,14 +587,14 @@ constexpr int kSlab = 256;
 template <int RB>
 struct GradCfg {
   static constexpr int kStages = RB == 1 ? 2 : 3;
-  static constexpr int kVecWarps = 4, kMmaWarp = kVecWarps + kProdWarps;
+  static constexpr int kVecWarps = 8, kMmaWarp = kVecWarps + kProdWarps;
   static constexpr int kThreads = (kMmaWarp + 1) * 32;
   static constexpr int kRows = 64 * kSlab * 2;             // four blocks of 64 rows x 128 bytes
   static constexpr int kPart = RB * kBlockBytes;           // one 16-bit part of the vectors
   static constexpr int kStageBytes = kRows + 2 * kPart;
   static constexpr int kTmemCols = RB == 1 ? 128 : 256;    // two sums of 64 RB columns
   static constexpr int kPerSm = RB == 1 ? 2 : 1;
-  static constexpr int kBars = 2 * kStages + 1;
+  static constexpr int kBars = 3 * kStages + 1;
   static constexpr int kSums = kSlab * 64 * RB * 4;        // over the ring, once it is drained
   static_assert(kSums <= kStages * kStageBytes, "the sums lie over the ring");
   static constexpr int kSmem = 1024 + kStages * kStageBytes + 8 * kBars + 64;
@@ -608,8 +609,41 @@ struct GradParams {
   int slabs_a, slabs;     // slabs of x, of both
 };
 
+// Adds up the S parts [rank16][256 / S] fp32 of a share of a slab's columns at `sums`, in order, and writes them, 8 numbers that lie
+// together in the result at a time.
+template <typename T, int S, int THREADS>
+__device__ __forceinline__ void add_parts(const LoraWeightGrad& p, uint32_t sums, int rank16, bool is_a, int adapter, int64_t col0) {
+  constexpr int kCols = kSlab / S;
+  const int64_t width = is_a ? p.k : p.n;
+  T* out = static_cast<T*>(is_a ? p.d_a : p.d_b) + static_cast<int64_t>(adapter) * p.rank * width;
+  const int items = p.rank * kCols / 8;
+  for (int e = threadIdx.x; e < items; e += THREADS) {
+    // 8 columns of a rank, or 8 ranks of a column
+    const int j = is_a ? e / (kCols / 8) : e / kCols * 8, m = is_a ? e % (kCols / 8) * 8 : e % kCols;
+    if (col0 + m >= width) continue;
+    float v[8] = {};
+#pragma unroll
+    for (int c = 0; c < S; ++c) {
+      const uint32_t at = sums + ((c * rank16 + j) * kCols + m) * 4;
+      if (is_a) {
+        const uint4 x = ld_shared_v4(at), y = ld_shared_v4(at + 16);
+        const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += __uint_as_float(w[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += ld_shared_f32(at + i * kCols * 4);
+      }
+    }
+    *reinterpret_cast<uint4*>(out + (is_a ? j * width + col0 + m : (col0 + m) * p.rank + j)) =
+        make_uint4(Pair<T>::pack(v[0], v[1]), Pair<T>::pack(v[2], v[3]), Pair<T>::pack(v[4], v[5]), Pair<T>::pack(v[6], v[7]));
+  }
+}
+
 template <typename T, int RB>
-__global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lora_weight_grad_kernel(const __grid_constant__ GradParams q) {
+__global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lora_weight_grad_kernel(const __grid_constant__ GradParams q,
+                                                                                                       const __grid_constant__ CUtensorMap map_x,
+                                                                                                       const __grid_constant__ CUtensorMap map_d_out) {
   using C = GradCfg<RB>;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   const LoraWeightGrad& p = q.p;
@@ -617,9 +651,10 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
   const uint32_t ring = smem_u32(smem);
   uint64_t* bar_mem = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes);
   const uint32_t bars = smem_u32(bar_mem);
-  const auto full = [&](int s) { return bars + 8u * s; };
+  const auto full = [&](int s) { return bars + 8u * s; };   // the vectors are there, and rows that were copied one by one
   const auto freed = [&](int s) { return bars + 8u * (C::kStages + s); };
-  const uint32_t bar_sums = bars + 8u * (2 * C::kStages);
+  const auto landed = [&](int s) { return bars + 8u * (2 * C::kStages + s); };   // and rows by TMA
+  const uint32_t bar_sums = bars + 8u * (3 * C::kStages);
   volatile uint32_t* words = reinterpret_cast<volatile uint32_t*>(bar_mem + C::kBars);
   const WaitCtx wctx{smem_u32(const_cast<uint32_t*>(words) + 1), q.fault_word};
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -631,14 +666,13 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
   const bool is_a = slab < q.slabs_a;
   const int64_t col0 = static_cast<int64_t>(is_a ? slab : slab - q.slabs_a) * kSlab;
   const int64_t width = is_a ? p.k : p.n;
-  const T* rows = static_cast<const T*>(is_a ? p.x : p.d_out);
-  const int64_t ld = is_a ? p.ld_x : p.ld_d_out;
   const float* vecs = is_a ? p.g : p.h;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
-      mbar_init(full(s), (C::kVecWarps + kProdWarps) * 32);
+      mbar_init(full(s), C::kVecWarps / 2 * 32 + kProdThreads);
       mbar_init(freed(s), 1);
+      mbar_init(landed(s), 1);
     }
     mbar_init(bar_sums, 1);
     words[1] = 0u;
@@ -665,34 +699,55 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
   float up = 1.f;
 
   if (warp >= C::kVecWarps && warp < C::kMmaWarp) {
-    // ---- copies: a warp takes every fourth row, a lane 16 bytes of it ----
+    // ---- copies. 64 rows that lie together come by TMA; others one by one: a warp takes every fourth, a lane 16 bytes of it ----
     const int w = warp - C::kVecWarps;
+    const int64_t ld = is_a ? p.ld_x : p.ld_d_out;
+    const T* rows = static_cast<const T*>(is_a ? p.x : p.d_out);
     const int64_t col = col0 + lane * 8;
     const bool in_width = col < width;
     const T* src = rows + (in_width ? col : 0);
     const uint32_t dst0 = ring + (lane >> 3) * kBlockBytes + w * 128;
     // (row w + 4 i: its swizzle is (w + 4 i) & 7)
     const uint32_t even = ((lane & 7) ^ w) << 4, odd = ((lane & 7) ^ (w + 4)) << 4;
-    int32_t mine = n > 0 ? row_at(chunk0, w + 4 * (lane & 15)) : -1;   // lane i < 16: row w + 4 i
+    int32_t lo = n > 0 ? row_at(chunk0, lane) : -1, hi = n > 0 ? row_at(chunk0, lane + 32) : -1;   // the chunk's rows
+    int it = 0;
+    bool ok = true;
 #pragma unroll 1
-    for (int it = 0; it < n; ++it) {
+    for (; it < n; ++it) {
       const int s = it % C::kStages;
-      if (it >= C::kStages && !mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x41)) break;
-      const int32_t now = mine;
-      if (it + 1 < n) mine = row_at(chunk0 + it + 1, w + 4 * (lane & 15));
-      const uint32_t dst = dst0 + s * C::kStageBytes;
+      if (it >= C::kStages && !(ok = mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x41))) break;
+      const int32_t row0 = __shfl_sync(0xffffffffu, lo, 0), now_lo = lo, now_hi = hi;
+      const bool together = __all_sync(0xffffffffu, lo >= 0 && lo == row0 + lane && hi == row0 + 32 + lane);
+      if (it + 1 < n) {
+        lo = row_at(chunk0 + it + 1, lane);
+        hi = row_at(chunk0 + it + 1, lane + 32);
+      }
+      const uint32_t dst = ring + s * C::kStageBytes;
+      if (together) {
+        if (w == 0 && lane == 0) {
+          mbar_arrive_expect_tx(landed(s), C::kRows);
+#pragma unroll
+          for (int i = 0; i < kSlab / 64; ++i)
+            tma_load_2d(dst + i * kBlockBytes, is_a ? &map_x : &map_d_out, landed(s), static_cast<int>(col0) + i * 64, row0);
+        }
+        mbar_arrive(full(s));
+        continue;
+      }
+      if (w == 0 && lane == 0) mbar_arrive(landed(s));
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int32_t row = __shfl_sync(0xffffffffu, now, i);
+        const int32_t row = __shfl_sync(0xffffffffu, i < 8 ? now_lo : now_hi, (w + 4 * i) & 31);
         const bool take = in_width && row >= 0;
-        cp_async16(dst + i * 512 + (i & 1 ? odd : even), take ? src + row * ld : rows, take);
+        cp_async16(dst0 + s * C::kStageBytes + i * 512 + (i & 1 ? odd : even), take ? src + row * ld : rows, take);
       }
       cp_async_arrive(full(s));
     }
     cp_async_wait_all();
-  } else if (warp < 4) {
-    // ---- vectors: a thread takes 8 ranks of every (16 / RB)-th row ----
-    const int t = threadIdx.x;
+    if (!ok)   // (and for copies by TMA)
+      for (int i = it - C::kStages; i < it; ++i) mbar_wait(wctx, landed(i % C::kStages), (i / C::kStages) & 1, 0x45);
+  } else if (warp < C::kVecWarps) {
+    // ---- vectors: the two halves of the warps take the chunks in turn, a thread 8 ranks of every (16 / RB)-th row ----
+    const int turn = warp / (C::kVecWarps / 2), t = threadIdx.x % (C::kVecWarps * 16);
     const int c8 = t % (8 * RB), r0 = t / (8 * RB);
     constexpr int kStep = 16 / RB, kMine = 64 / kStep;
     const bool used = c8 * 8 < q.rank16, has = c8 * 8 < p.rank;
@@ -719,13 +774,13 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
       }
     };
     bool ok = true;
-    if (n > 0) {
-      find(chunk0);
+    if (turn < n) {
+      find(chunk0 + turn);
       load();
-      if (n > 1) find(chunk0 + 1);
+      if (turn + 2 < n) find(chunk0 + turn + 2);
     }
 #pragma unroll 1
-    for (int it = 0; it < n; ++it) {
+    for (int it = turn; it < n; it += 2) {
       const int s = it % C::kStages;
       if (it >= C::kStages && !(ok = mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x42))) break;
       const uint32_t dst = ring + s * C::kStageBytes + C::kRows + (c8 >> 3) * kBlockBytes;
@@ -749,8 +804,8 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
       }
       fence_async_shared();
       mbar_arrive(full(s));
-      if (it + 1 < n) load();
-      if (it + 2 < n) find(chunk0 + it + 2);
+      if (it + 2 < n) load();
+      if (it + 4 < n) find(chunk0 + it + 4);
     }
   } else if (n > 0) {
     // ---- tensor cores ----
@@ -758,6 +813,7 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
     for (int it = 0; it < n; ++it) {
       const int s = it % C::kStages;
       if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x43))) break;
+      if (!(ok = mbar_wait(wctx, landed(s), (it / C::kStages) & 1, 0x46))) break;
       fence_async_shared();
       tc_fence_after_sync();
       const uint32_t a = ring + s * C::kStageBytes, b = a + C::kRows;
@@ -777,75 +833,46 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
     if (ok) tc_commit_elect(bar_sums);
   }
 
-  // sums [rank][256 columns] fp32 over the ring
-  if (warp < 4) {
-    const int blocks = q.rank16 / 16;
-    const bool have = n > 0 && mbar_wait_long(wctx, bar_sums, 0, 0x44);
-    tc_fence_after_sync();
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp) << 21);
-    const float c = is_a ? up : up * __ldg(p.scales + adapter);
-    for (int half = 0; half < 2; ++half)
-      for (int b = 0; b < blocks; ++b) {
-        uint32_t x[16];
-        if (have) {
-          tmem_ld(lanes + half * 64 * RB + b * 16, x);
-          tmem_wait_ld(x);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          st_shared_f32(ring + ((b * 16 + i) * kSlab + half * 128 + threadIdx.x) * 4, have ? c * __uint_as_float(x[i]) : 0.f);
-      }
-  }
+  // The cluster's CTAs share the slab's columns: every CTA leaves its sums of a share in the ring of the CTA that adds them up, once
+  // all rings are drained.
+  const bool have = warp < C::kVecWarps && n > 0 && mbar_wait_long(wctx, bar_sums, 0, 0x44);
   __syncwarp();
-  tc_fence_before_sync();
   if (S > 1) cluster_sync();
   else __syncthreads();
-  // the cluster's CTAs share the slab's columns; 8 numbers that lie together in the result at a time
-  const int cols = kSlab >> q.cluster_log;   // a multiple of 8
-  const int64_t factor = static_cast<int64_t>(adapter) * p.rank * width;
-  const auto sum_at = [&](int j, int m, int cta) {
-    return cluster_map_shared(ring + (j * kSlab + m) * 4, cta);
-  };
-  if (is_a) {
-    T* out = static_cast<T*>(p.d_a) + factor;
-    for (int e = threadIdx.x; e < p.rank * (cols / 8); e += C::kThreads) {
-      const int j = e / (cols / 8), m = rank * cols + (e % (cols / 8)) * 8;
-      if (col0 + m >= width) continue;
-      float f[8] = {};
-      for (int cta = 0; cta < S; ++cta) {
-        const float4 a = ld_shared_cluster_f4(sum_at(j, m, cta)), b = ld_shared_cluster_f4(sum_at(j, m + 4, cta));
-        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
-        f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+  const int cols = kSlab >> q.cluster_log;   // at least 32: a warp's columns belong to one CTA
+  if (warp < C::kVecWarps) {
+    tc_fence_after_sync();
+    const int half = warp >> 2, col = threadIdx.x & (cols - 1);
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * 64 * RB;
+    const uint32_t to = cluster_map_shared(ring + (rank * q.rank16 * cols + col) * 4, threadIdx.x / cols);
+    const float c = is_a ? up : up * __ldg(p.scales + adapter);
+    for (int b = 0; b < q.rank16 / 16; ++b) {
+      uint32_t x[16];
+      if (have) {
+        tmem_ld(lanes + b * 16, x);
+        tmem_wait_ld(x);
       }
-      *reinterpret_cast<uint4*>(out + j * width + col0 + m) =
-          make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]), Pair<T>::pack(f[6], f[7]));
-    }
-  } else {
-    T* out = static_cast<T*>(p.d_b) + factor;
-    for (int e = threadIdx.x; e < p.rank / 8 * cols; e += C::kThreads) {
-      const int j = e / cols * 8, m = rank * cols + e % cols;
-      if (col0 + m >= width) continue;
-      float f[8] = {};
-      for (int cta = 0; cta < S; ++cta)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float v;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sum_at(j + i, m, cta)) : "memory");
-          f[i] += v;
-        }
-      *reinterpret_cast<uint4*>(out + (col0 + m) * p.rank + j) =
-          make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]), Pair<T>::pack(f[6], f[7]));
+      for (int i = 0; i < 16; ++i)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (b * 16 + i) * cols * 4), "f"(have ? c * __uint_as_float(x[i]) : 0.f)
+                     : "memory");
     }
+    tc_fence_before_sync();
   }
   __syncwarp();
-  if (S > 1) cluster_sync();   // (nobody reads this CTA's sums any more)
+  if (S > 1) cluster_sync();
   else __syncthreads();
   tc_fence_after_sync();
   if (warp == C::kMmaWarp) tmem_dealloc(tmem, C::kTmemCols);
+  const int64_t mine = col0 + rank * cols;
+  if (S == 8) add_parts<T, 8, C::kThreads>(p, ring, q.rank16, is_a, adapter, mine);
+  else if (S == 4) add_parts<T, 4, C::kThreads>(p, ring, q.rank16, is_a, adapter, mine);
+  else if (S == 2) add_parts<T, 2, C::kThreads>(p, ring, q.rank16, is_a, adapter, mine);
+  else add_parts<T, 1, C::kThreads>(p, ring, q.rank16, is_a, adapter, mine);
 }
 
 template <typename T, int RB>
-ks_status_t launch_grad(const char* where, const GradParams& q, int64_t items, cudaStream_t stream) {
+ks_status_t launch_grad(const char* where, const GradParams& q, const CUtensorMap (&maps)[2], int64_t items, cudaStream_t stream) {
   using C = GradCfg<RB>;
   static std::mutex mu;
   static bool done[64] = {};
@@ -860,7 +887,7 @@ ks_status_t launch_grad(const char* where, const GradParams& q, int64_t items, c
     }
   }
   launch_programmatic_cluster(lora_weight_grad_kernel<T, RB>, static_cast<unsigned>(items << q.cluster_log), 1u << q.cluster_log,
-                              true, C::kThreads, C::kSmem, stream, q);
+                              true, C::kThreads, C::kSmem, stream, q, maps[0], maps[1]);
   KSB_CHECK_LAUNCH(where);
   return KS_SUCCESS;
 }
@@ -917,9 +944,20 @@ ks_status_t lora_weight_grad_pass(const char* where, const LoraWeightGrad& p, ks
   const int64_t room = static_cast<int64_t>(sm_count()) * (wide ? 1 : 2);
   while ((2 << q.cluster_log) <= kMaxCluster && items << (q.cluster_log + 1) <= room && p.rows > 64 << q.cluster_log) ++q.cluster_log;
   if (items << q.cluster_log > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
+  CUtensorMap maps[2] = {};
+  if (p.rows > 0) {   // (without rows nothing is copied)
+    const auto encode = [&](CUtensorMap* m, const void* base, int64_t width, int64_t ld) {
+      const uint64_t dims[2] = {static_cast<uint64_t>(width), static_cast<uint64_t>(p.rows)}, stride = static_cast<uint64_t>(ld) * 2;
+      const uint32_t box[2] = {64, 64};
+      return tma_encode(m, dtype == KS_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, &stride,
+                        box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (!encode(&maps[0], p.x, p.k, p.ld_x) || !encode(&maps[1], p.d_out, p.n, p.ld_d_out))
+      KSB_FAIL(KS_ERROR_INTERNAL, std::string(where) + ": tensor map rejected");
+  }
   if (dtype == KS_DTYPE_F16)
-    return wide ? launch_grad<__half, 2>(where, q, items, stream) : launch_grad<__half, 1>(where, q, items, stream);
-  return wide ? launch_grad<__nv_bfloat16, 2>(where, q, items, stream) : launch_grad<__nv_bfloat16, 1>(where, q, items, stream);
+    return wide ? launch_grad<__half, 2>(where, q, maps, items, stream) : launch_grad<__half, 1>(where, q, maps, items, stream);
+  return wide ? launch_grad<__nv_bfloat16, 2>(where, q, maps, items, stream) : launch_grad<__nv_bfloat16, 1>(where, q, maps, items, stream);
 }
 
 }  // namespace sm100
