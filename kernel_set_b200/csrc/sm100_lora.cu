@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
           }
         }
         // second product: y0 + c D in the stage that holds y0, then out: of the quarter's 32 rows a warp stores 16, 128 bytes of each
-        // (the two halves' 64 bytes apart: 106 us against ... for 16384 rows beside 4096 x 4096)
+        // (each half its 64 bytes: 106 us against 83 for 16384 rows beside 4096 x 4096)
         const float c = s * up;
         const int piece = lane & 7, out_row = quarter * 32 + half * 16 + (lane >> 3);
         T* dst[4];
@@ -942,7 +942,13 @@ ks_status_t lora_weight_grad_pass(const char* where, const LoraWeightGrad& p, ks
   const bool wide = p.rank > 64;
   const int64_t items = static_cast<int64_t>(p.adapters) * q.slabs;
   const int64_t room = static_cast<int64_t>(sm_count()) * (wide ? 1 : 2);
-  while ((2 << q.cluster_log) <= kMaxCluster && items << (q.cluster_log + 1) <= room && p.rows > 64 << q.cluster_log) ++q.cluster_log;
+  // CTAs of a slab: as many as run at a time, and twice that where four chunks are left to each, since adapters without rows
+  // leave SMs idle (16384 rows, 4 of 8 adapters, rank 64: 154 us for both launches against 194; all 8 158 / 161; 2 of 2 158 / 149)
+  const auto worth = [&](int log) {
+    const int64_t ctas = items << log;
+    return p.rows > 32 << log && (ctas <= room || (ctas <= 2 * room && p.rows / p.adapters >= 128 << log));
+  };
+  while ((2 << q.cluster_log) <= kMaxCluster && worth(q.cluster_log + 1)) ++q.cluster_log;
   if (items << q.cluster_log > INT32_MAX) KSB_FAIL(KS_ERROR_UNSUPPORTED_SHAPE, std::string(where) + ": grid exceeds CUDA grid limits");
   CUtensorMap maps[2] = {};
   if (p.rows > 0) {   // (without rows nothing is copied)

@@ -311,3 +311,51 @@ def test_experts_adapters_on_a_routed_layers_rows(ks, cuda):
     out = ks.lora.apply(torch.empty_like(p.base), p.base[o].contiguous(), p.x[o].contiguous(), p.a, p.b, p.scales, None, offsets[:-1].contiguous())
     want, bound, _, _ = p.forward()
     check("out", out, want[o], bound[o])
+
+
+@pytest.mark.parametrize("rank", [16, 64, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_sequences_beside_rows_that_are_not_numbers(ks, cuda, rank, dtype):
+    """Runs of rows of one adapter, of odd lengths, with NaN and infinities in the rows between and behind them, as columns of wider
+    tensors; with the rows' numbers and without, to the bit."""
+    lengths = [(0, 200), (1, 64), (2, 63), (4, 129), (5, 70)]       # adapters 3 and 5: no row, rows that no longer count
+    ids = torch.cat([torch.full((n,), a) for a, n in lengths])
+    p = Problem(ids.numel(), 5, rank, 328, 520, dtype, seed=7)
+    p.ids = torch.where(ids < 5, ids, -1).to(torch.int32).to(cuda)
+    none = p.ids < 0
+    _, _, h, _ = p.forward()
+    hf = h.float()
+    want, bounds = p.backward(hf)
+    x, d_out, d_x = (torch.full((p.tokens, w + 64), float("nan"), dtype=dtype, device=cuda) for w in (p.k, p.n, p.k))
+    x[:, 8:8 + p.k], d_out[:, 16:16 + p.n] = p.x, p.d_out
+    x[none], d_out[none] = float("nan"), float("inf")
+    hf[none] = float("nan")
+    ids, offsets = _plan(ks, p)
+    results = []
+    for order in (ids, None):
+        d_a, d_b = torch.full_like(p.a, 9.0), torch.full_like(p.b, 9.0)
+        ks.lora.backward(d_x[:, 24:24 + p.k], d_a, d_b, p.d_x_base, d_out[:, 16:16 + p.n], x[:, 8:8 + p.k], hf, p.a, p.b, p.scales, order, offsets)
+        results.append((d_x[:, 24:24 + p.k].clone(), d_a, d_b))
+    for what, got, w, b in zip(("d_x", "d_a", "d_b"), results[0], want, bounds):
+        check(what, got, w, b)
+    assert torch.equal(results[0][0][none], p.d_x_base[none])
+    assert not results[0][1][3].any() and not results[0][2][3].any()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("tokens,adapters,active", [(4096, 2, 1), (5000, 8, 3), (3000, 6, 6)])
+def test_backward_of_long_batches(ks, cuda, tokens, adapters, active):
+    """Slabs whose rows several CTAs share, some adapters without rows; every run gives the same bits."""
+    p = Problem(tokens, adapters, 16, 1024, 768, seed=9, active=active)
+    ids, offsets = _plan(ks, p)
+    _, _, h, _ = p.forward()
+    hf = h.float()
+    want, bounds = p.backward(hf)
+    first = None
+    for _ in range(3):
+        got = ks.lora.backward(torch.empty_like(p.x), torch.empty_like(p.a), torch.empty_like(p.b), p.d_x_base, p.d_out, p.x, hf, p.a, p.b,
+                               p.scales, ids, offsets)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
+    for what, x, y, b in zip(("d_x", "d_a", "d_b"), first, want, bounds):
+        check(what, x, y, b)
