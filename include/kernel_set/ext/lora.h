@@ -48,7 +48,8 @@ KS_API ks_status_t ks_lora_plan(int32_t* sorted_ids, int32_t* offsets,
  * With ks_moe_compute_permutation's offsets and sorted_ids = NULL the rows of a routed
  * layer that are sorted by expert get their expert's adapter.
  * fp32 accumulation, one rounding to `dtype`; A x enters the second product as a sum of two 16-bit
- * numbers (2^-16 relative in bf16) or in fp32. rank at most 4096.
+ * numbers (2^-16 relative in bf16) or in fp32. A row whose A x is not finite gets NaN where
+ * it would get infinities. rank at most 4096.
  */
 KS_API ks_status_t ks_lora_apply(void* out, int64_t ld_out, const void* base,
                                  int64_t ld_base, float* h, const void* x,

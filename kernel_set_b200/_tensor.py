@@ -111,11 +111,13 @@ def default_stream(stream: TensorLike, reference: TensorLike = None) -> int:
 
 
 _HERE = contextlib.nullcontext()
+# (current_device() first looks whether CUDA is initialised, which it is where there is a CUDA tensor: 0.4 us)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def on_device_of(obj: TensorLike):
     """A context in which the device of ``obj`` is the current one (the library launches on the current device)."""
-    if isinstance(obj, torch.Tensor) and obj.is_cuda and obj.device.index != torch.cuda.current_device():
+    if isinstance(obj, torch.Tensor) and obj.is_cuda and obj.device.index != _current_device():
         return torch.cuda.device(obj.device)
     return _HERE
 
@@ -126,6 +128,16 @@ def same_dtype(reference: TensorLike, **others: TensorLike) -> None:
         for name, t in others.items():
             if isinstance(t, torch.Tensor) and t.dtype != reference.dtype:
                 raise ValueError(f"{name} must be {reference.dtype}, as the other tensors of the call; got {t.dtype}")
+
+
+def at_least(numel: int, dtype: Optional[torch.dtype], **tensors: TensorLike) -> None:
+    """Refuses tensors of fewer than ``numel`` elements or of another type (raw addresses have neither)."""
+    for name, t in tensors.items():
+        if isinstance(t, torch.Tensor):
+            if dtype is not None and t.dtype is not dtype:
+                raise ValueError(f"{name} must be {dtype}; got {t.dtype}")
+            if t.numel() < numel:
+                raise ValueError(f"{name}: {t.numel()} elements where {numel} are expected")
 
 
 def infer_dtype(reference: TensorLike, dtype: Optional[int]) -> int:

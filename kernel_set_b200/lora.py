@@ -147,7 +147,9 @@ def backward(d_x: torch.Tensor, d_a: torch.Tensor, d_b: torch.Tensor, d_x_base: 
             and d_b.shape == (adapters, n, rank) and h.shape == (tokens, rank) and scales.shape == (adapters,)
             and d_x.dtype is d_x_base.dtype is d_out.dtype is a.dtype is d_a.dtype is b.dtype is d_b.dtype is dt
             and h.dtype is scales.dtype is torch.float32
-            and all(t.is_cuda for t in (d_x, d_x_base, d_out, x)) and all(t.is_cuda and t.is_contiguous() for t in (a, d_a, b, d_b, h, scales))
+            and d_x.is_cuda and d_x_base.is_cuda and d_out.is_cuda and x.is_cuda and a.is_cuda and d_a.is_cuda and b.is_cuda and d_b.is_cuda
+            and h.is_cuda and scales.is_cuda and a.is_contiguous() and d_a.is_contiguous() and b.is_contiguous() and d_b.is_contiguous()
+            and h.is_contiguous() and scales.is_contiguous()
             and (ld_d_x := _ld(d_x, tokens, k)) >= 0 and (ld_d_x_base := _ld(d_x_base, tokens, k)) >= 0
             and (ld_d_out := _ld(d_out, tokens, n)) >= 0 and (ld_x := _ld(x, tokens, k)) >= 0
             and _plan_ok(sorted_ids, offsets, tokens, adapters)):

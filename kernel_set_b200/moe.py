@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from ._lib import by_address as lib, check
-from ._tensor import TensorLike, default_stream, dtype_to_ks, f32_ptr, i32_ptr, infer_dtype, on_device_of, ptr, same_dtype
+from ._tensor import TensorLike, at_least, default_stream, dtype_to_ks, f32_ptr, i32_ptr, infer_dtype, on_device_of, ptr, same_dtype
 
 
 def grouped_gemm(c: TensorLike, a: TensorLike, b: TensorLike, expert_offsets: TensorLike, num_experts: int,
@@ -123,7 +123,18 @@ def unpermute_backward(d_permuted: TensorLike, d_weights: TensorLike, d_out: Ten
     ``d_weights[t,k] = <d_out[t], permuted[r]>`` (fp32). Rows without a pair and pairs without a row get zeros; a pair may
     occur once in ``sorted_token_ids``. ``d_permuted`` may be ``permuted``. Returns ``(d_permuted, d_weights)``."""
     dt = infer_dtype(permuted, dtype)
-    same_dtype(permuted, d_permuted=d_permuted, d_out=d_out)
+    pairs = num_tokens * top_k
+    # one quick test of types and sizes, the message where it fails
+    if not (type(d_permuted) is type(permuted) is type(d_out) is type(d_weights) is type(routing_weights) is type(sorted_token_ids)
+            is torch.Tensor and d_permuted.dtype is d_out.dtype is permuted.dtype and d_weights.dtype is routing_weights.dtype is torch.float32
+            and sorted_token_ids.dtype is torch.int32 and d_weights.numel() >= pairs and routing_weights.numel() >= pairs
+            and sorted_token_ids.numel() >= pairs and d_permuted.numel() >= pairs * hidden and permuted.numel() >= pairs * hidden
+            and d_out.numel() >= num_tokens * hidden):
+        same_dtype(permuted, d_permuted=d_permuted, d_out=d_out)
+        at_least(pairs, torch.float32, d_weights=d_weights, routing_weights=routing_weights)
+        at_least(pairs, torch.int32, sorted_token_ids=sorted_token_ids)
+        at_least(pairs * hidden, None, d_permuted=d_permuted, permuted=permuted)
+        at_least(num_tokens * hidden, None, d_out=d_out)
     with on_device_of(permuted):
         check(lib.ks_moe_unpermute_backward(ptr(d_permuted, name="d_permuted"), f32_ptr(d_weights, name="d_weights"),
                                             ptr(d_out, name="d_out"), ptr(permuted, name="permuted"),
@@ -138,7 +149,14 @@ def permute_backward(d_input: TensorLike, d_permuted: TensorLike, sorted_token_i
     """Gradient of :func:`permute`: ``d_input[t]`` is the sum of token ``t``'s rows of ``d_permuted``, in slot order, in
     fp32; a pair may occur once in ``sorted_token_ids``."""
     dt = infer_dtype(d_permuted, dtype)
-    same_dtype(d_permuted, d_input=d_input)
+    pairs = num_tokens * top_k
+    if not (type(d_input) is type(d_permuted) is type(sorted_token_ids) is torch.Tensor and d_input.dtype is d_permuted.dtype
+            and sorted_token_ids.dtype is torch.int32 and sorted_token_ids.numel() >= pairs and d_permuted.numel() >= pairs * hidden
+            and d_input.numel() >= num_tokens * hidden):
+        same_dtype(d_permuted, d_input=d_input)
+        at_least(pairs, torch.int32, sorted_token_ids=sorted_token_ids)
+        at_least(pairs * hidden, None, d_permuted=d_permuted)
+        at_least(num_tokens * hidden, None, d_input=d_input)
     with on_device_of(d_permuted):
         check(lib.ks_moe_permute_backward(ptr(d_input, name="d_input"), ptr(d_permuted, name="d_permuted"),
                                           i32_ptr(sorted_token_ids, name="sorted_token_ids"), int(num_tokens), int(top_k),
@@ -152,7 +170,15 @@ def gate_softmax_topk_backward(d_logits: TensorLike, d_weights: TensorLike, weig
     """Gradient of :func:`gate_softmax_topk` with respect to the logits. ``weights`` and ``indices`` are what the gate
     gave; ``logits`` may be ``None`` with ``renormalize``. ``d_logits`` may be ``logits``."""
     dt = infer_dtype(d_logits, dtype)
-    same_dtype(d_logits, logits=logits)
+    pairs, numel = num_tokens * top_k, num_tokens * num_experts
+    if not (type(d_logits) is type(d_weights) is type(weights) is type(indices) is torch.Tensor
+            and d_weights.dtype is weights.dtype is torch.float32 and indices.dtype is torch.int32 and d_weights.numel() >= pairs
+            and weights.numel() >= pairs and indices.numel() >= pairs and d_logits.numel() >= numel
+            and (logits is None or (type(logits) is torch.Tensor and logits.dtype is d_logits.dtype and logits.numel() >= numel))):
+        same_dtype(d_logits, logits=logits)
+        at_least(pairs, torch.float32, d_weights=d_weights, weights=weights)
+        at_least(pairs, torch.int32, indices=indices)
+        at_least(numel, None, d_logits=d_logits, logits=logits)
     with on_device_of(d_logits):
         check(lib.ks_moe_gate_softmax_topk_backward(ptr(d_logits, name="d_logits"), f32_ptr(d_weights, name="d_weights"),
                                                     f32_ptr(weights, name="weights"), i32_ptr(indices, name="indices"),

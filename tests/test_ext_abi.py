@@ -116,3 +116,22 @@ def test_python_wrappers_refuse(ks):
         ks.lora.plan(torch.zeros(3, dtype=torch.int64), 2)
     with pytest.raises(ValueError, match="must be"):
         ks.moe.permute_backward(torch.zeros(2, 8), torch.zeros(4, 8, dtype=bf), ids, 2, 2, 8)
+
+
+def test_moe_backward_wrappers_refuse(ks):
+    """Types and sizes that would be read as something else, or beyond the end (torch.topk's indices are 64-bit, for one)."""
+    f, i = torch.zeros(4, 2), torch.zeros(8, dtype=torch.int32)
+    rows, pairs = torch.zeros(4, 8), torch.zeros(8, 8)
+    up = dict(d_permuted=pairs, d_weights=f, d_out=rows, permuted=pairs, sorted_token_ids=i, routing_weights=f, num_tokens=4, top_k=2, hidden=8)
+    pb = dict(d_input=rows, d_permuted=pairs, sorted_token_ids=i, num_tokens=4, top_k=2, hidden=8)
+    gb = dict(d_logits=rows, d_weights=f, weights=f, indices=i, logits=rows, num_tokens=4, num_experts=8, top_k=2)
+    for fn, good, bad in ((ks.moe.unpermute_backward, up, (dict(d_weights=f.half()), dict(routing_weights=f[:3]), dict(sorted_token_ids=i.long()),
+                                                           dict(permuted=pairs[:7]), dict(d_out=rows[:3]), dict(d_permuted=pairs.half()))),
+                          (ks.moe.permute_backward, pb, (dict(sorted_token_ids=i[:7]), dict(d_permuted=pairs[:7]), dict(d_input=rows[:3]))),
+                          (ks.moe.gate_softmax_topk_backward, gb, (dict(indices=i.long()), dict(weights=f.double()), dict(d_weights=f[:3]),
+                                                                   dict(logits=rows[:3]), dict(d_logits=rows.half())))):
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            fn(**good)
+        for b in bad:
+            with pytest.raises(ValueError, match="must be torch|elements where"):
+                fn(**{**good, **b})
