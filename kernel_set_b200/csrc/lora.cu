@@ -18,7 +18,10 @@ namespace {
 
 constexpr int kMaxAnyRank = 4096;
 constexpr int kAnyThreads = 256;
-constexpr int kFewRows = 256;   // up to which the forward pass takes 8 rows at a time
+// Rows up to which the forward pass takes 8 to 32 at a time instead of tiles of 128, by rank (us cold, few / tiles): rank 16, 512 rows of 64
+// adapters beside 4096 x 14336 42 / 67, of one beside 4096 x 4096 19.5 / 22.6; rank 32, 700 rows of 64 34 / 34, 1024 rows 38 / 34;
+// rank 64, 300 rows of 8 30 / 24, 512 of 64 44 / 38.
+constexpr int few_rows(int rank) { return rank <= 32 ? 512 : 256; }
 
 // Any rank, widths and alignment: a CTA per place. The warps take the ranks in turn, a lane every 32nd product of a
 // sum; then a thread takes every 256th output.
@@ -88,7 +91,7 @@ __global__ void __launch_bounds__(kAnyThreads) lora_weight_grad_any_kernel(LoraW
 
 ks_status_t run_pass(const char* where, const LoraPass& p, bool forward, ks_dtype_t dtype, cudaStream_t s) {
   if (sm100::lora_tile_takes(p)) {
-    if (forward && p.rows <= kFewRows) return sm100::lora_few_pass(where, p, dtype, s);
+    if (forward && p.rows <= few_rows(p.rank)) return sm100::lora_few_pass(where, p, dtype, s);
     return sm100::lora_tile_pass(where, p, forward, dtype, s);
   }
   const unsigned grid = static_cast<unsigned>(p.rows);

@@ -27,6 +27,9 @@ SHAPES = [
     (513, 2, 20, 100, 60, BF, 0.5, 2),           # widths of 4 elements only
     (600, 3, 256, 256, 128, HF, 0.0, 3),         # a rank beyond 128
     (2050, 7, 96, 768, 640, BF, 0.1, 6),
+    (500, 3, 32, 264, 520, HF, 0.1, 3),
+    (512, 200, 16, 128, 72, BF, 0.2, 150),
+    (513, 200, 16, 128, 72, BF, 0.2, 150),
 ]
 
 
