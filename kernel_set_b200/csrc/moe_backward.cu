@@ -340,7 +340,7 @@ permute_backward_bulk_kernel(T* __restrict__ d_input, const T* __restrict__ d_pe
       row = row_of(ahead);
       const uint32_t mask = live[b];
       if (mask != 0u) {
-        ok = sm100::mbar_wait(wctx, bars + 8 * b, parity >> b & 1u, 0x51);
+        ok = sm100::all_lanes(sm100::mbar_wait(wctx, bars + 8 * b, parity >> b & 1u, 0x51));
         if (!ok) break;
         parity ^= 1u << b;
       }

@@ -114,6 +114,21 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Whether `ok` (the same for a warp) holds for both warps that share the named barrier `id`. Bounded waits end each on its own, so two
+// warps that meet at a barrier settle there whether both go on: one that left alone would leave the other at it for good.
+__device__ __forceinline__ bool pair_agrees(uint32_t id, bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "bar.red.and.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(all)
+      : "r"(id), "r"(ok ? 1u : 0u)
+      : "memory");
+  return all != 0u;
+}
+
 struct TileParams {
   LoraPass p;
   unsigned int* fault_word;
@@ -334,7 +349,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
       bool ok = true;
       for (int it = 0; it < n1; ++it) {
         const int s = it % C::kStages;
-        if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x33))) break;
+        if (!(ok = all_lanes(mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x33)))) break;
         fence_async_shared();
         tc_fence_after_sync();
         const uint32_t a = ring + s * C::kStageBytes, b = a + kRowsBytes;
@@ -348,12 +363,12 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         tc_commit_elect(free1(s));
       }
       if (ok && n1 > 0) tc_commit_elect(bar_sums);
-      if (ok && n2 > 0) ok = mbar_wait_long(wctx, bar_inner, 0, 0x34);
+      if (ok && n2 > 0) ok = all_lanes(mbar_wait_long(wctx, bar_inner, 0, 0x34));
       tc_fence_after_sync();
       for (int j = 0; ok && j < n2; ++j) {
         const int it = n1 + j, s = it % C::kStages, b = j & 1;
-        if (j >= 2 && !(ok = mbar_wait(wctx, out_free(b), ((j >> 1) - 1) & 1, 0x35))) break;
-        if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x36))) break;
+        if (j >= 2 && !(ok = all_lanes(mbar_wait(wctx, out_free(b), ((j >> 1) - 1) & 1, 0x35)))) break;
+        if (!(ok = all_lanes(mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x36)))) break;
         fence_async_shared();
         tc_fence_after_sync();
         const uint32_t w = ring + s * C::kStageBytes + kRowsBytes;
@@ -376,7 +391,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
       const bool used = quarter < quarters;   // (the quarters without rows only keep step)
       if (!joined) cluster_wait();
       joined = true;
-      bool ok = n1 == 0 || mbar_wait_long(wctx, bar_sums, 0, 0x37);
+      bool ok = n1 == 0 || all_lanes(mbar_wait_long(wctx, bar_sums, 0, 0x37));
       tc_fence_after_sync();
       if (ok && S > 1) {
         // ranks 4 j .. of row r at exchange + (j * 128 + r) * 16
@@ -395,7 +410,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         }
         __syncwarp();
         if (lane < S) mbar_arrive_cluster(bar_parts, lane);
-        ok = mbar_wait_cluster(wctx, bar_parts, 0, 0x38);
+        ok = all_lanes(mbar_wait_cluster(wctx, bar_parts, 0, 0x38));
         if (ok) {
           const int pieces = q.rank16 / 4 * quarters * 32;
           if (S == 2) reduce_scatter<2, C::kEpiWarps * 32>(exchange, pieces, quarters, rank);
@@ -403,9 +418,10 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
           else reduce_scatter<8, C::kEpiWarps * 32>(exchange, pieces, quarters, rank);
           __syncwarp();
           if (lane < S) mbar_arrive_cluster(bar_total, lane);
-          ok = mbar_wait_cluster(wctx, bar_total, 0, 0x3b);
+          ok = all_lanes(mbar_wait_cluster(wctx, bar_total, 0, 0x3b));
         }
       }
+      if (used) ok = pair_agrees(1 + quarter, ok);
       if (ok) {
         const auto sums_of = [&](int b, uint32_t (&x)[16]) {
           if (S > 1) {
@@ -492,13 +508,14 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         for (int j = 0; j < n2; ++j) {
           const int it = n1 + j, st = it % C::kStages, b = j & 1;
           const uint32_t tile = ring + st * C::kStageBytes;
-          if (!mbar_wait(wctx, full(st), (it / C::kStages) & 1, 0x3a)) break;
+          ok = all_lanes(mbar_wait(wctx, full(st), (it / C::kStages) & 1, 0x3a));
           uint4 y[4];
           if (used) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = ld_shared_v4(tile + r * 128 + (((half * 4 + i) ^ (r & 7)) << 4));
           }
-          if (!mbar_wait(wctx, out_full(b), (j >> 1) & 1, 0x39)) break;
+          ok = ok && all_lanes(mbar_wait(wctx, out_full(b), (j >> 1) & 1, 0x39));
+          if (!used && !ok) break;
           tc_fence_after_sync();
           if (used) {
             uint32_t d[32];
@@ -516,7 +533,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
               st_shared_v4(tile + r * 128 + (((half * 4 + i) ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
             }
             tc_fence_before_sync();
-            asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");   // (both halves of the quarter's rows are there)
+            if (!(ok = pair_agrees(1 + quarter, ok))) break;   // (both halves of the quarter's rows are there)
             const bool in_width = static_cast<int64_t>(out0 + j) * kChunk + piece * 8 < p.d_out;
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = ld_shared_v4(tile + (out_row + i * 4) * 128 + ((piece ^ ((out_row + i * 4) & 7)) << 4));
@@ -715,7 +732,7 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
 #pragma unroll 1
     for (; it < n; ++it) {
       const int s = it % C::kStages;
-      if (it >= C::kStages && !(ok = mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x41))) break;
+      if (it >= C::kStages && !(ok = all_lanes(mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x41)))) break;
       const int32_t row0 = __shfl_sync(0xffffffffu, lo, 0), now_lo = lo, now_hi = hi;
       const bool together = __all_sync(0xffffffffu, lo >= 0 && lo == row0 + lane && hi == row0 + 32 + lane);
       if (it + 1 < n) {
@@ -812,8 +829,8 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
     bool ok = true;
     for (int it = 0; it < n; ++it) {
       const int s = it % C::kStages;
-      if (!(ok = mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x43))) break;
-      if (!(ok = mbar_wait(wctx, landed(s), (it / C::kStages) & 1, 0x46))) break;
+      if (!(ok = all_lanes(mbar_wait(wctx, full(s), (it / C::kStages) & 1, 0x43)))) break;
+      if (!(ok = all_lanes(mbar_wait(wctx, landed(s), (it / C::kStages) & 1, 0x46)))) break;
       fence_async_shared();
       tc_fence_after_sync();
       const uint32_t a = ring + s * C::kStageBytes, b = a + C::kRows;
@@ -835,7 +852,7 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
 
   // The cluster's CTAs share the slab's columns: every CTA leaves its sums of a share in the ring of the CTA that adds them up, once
   // all rings are drained.
-  const bool have = warp < C::kVecWarps && n > 0 && mbar_wait_long(wctx, bar_sums, 0, 0x44);
+  const bool have = warp < C::kVecWarps && n > 0 && all_lanes(mbar_wait_long(wctx, bar_sums, 0, 0x44));
   __syncwarp();
   if (S > 1) cluster_sync();
   else __syncthreads();

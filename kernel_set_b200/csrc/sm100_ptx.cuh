@@ -129,6 +129,10 @@ __device__ __forceinline__ bool mbar_wait_long(const WaitCtx& ctx, uint32_t bar,
   }
 }
 
+// A wait's result for the whole warp. Every lane polls for itself, so when a limit runs out the lanes may end differently; a warp that goes
+// on to collectives (votes, shuffles, elected instructions, aligned barriers) goes on, or leaves, as one.
+__device__ __forceinline__ bool all_lanes(bool waited) { return __all_sync(0xffffffffu, waited); }
+
 // Waits for two barriers whose phases are usually both complete already: both are
 // tested before either result is used, so the two ~100-cycle round trips overlap.
 __device__ __forceinline__ bool mbar_wait_both(const WaitCtx& ctx, uint32_t bar_a, uint32_t parity_a, uint32_t code_a,
