@@ -47,8 +47,8 @@ KS_API ks_status_t ks_lora_plan(int32_t* sorted_ids, int32_t* offsets,
  *                offsets[num_adapters] on none. Values are clamped to [0, num_tokens].
  * With ks_moe_compute_permutation's offsets and sorted_ids = NULL the rows of a routed
  * layer that are sorted by expert get their expert's adapter.
- * fp32 accumulation, one rounding to `dtype`; A x enters the second product as a sum of two 16-bit
- * numbers (2^-16 relative in bf16) or in fp32. A row whose A x is not finite gets NaN where
+ * fp32 accumulation, one rounding to `dtype`; A x enters the second product in fp32 or as a sum of 16-bit
+ * numbers that hold it to 2^-24 of each element (bf16), 2^-22 (f16). A row whose A x is not finite gets NaN where
  * it would get infinities. rank at most 4096.
  */
 KS_API ks_status_t ks_lora_apply(void* out, int64_t ld_out, const void* base,

@@ -8,7 +8,7 @@
 //
 // Products by mma.m16n8k16 with the factor as the 16-row operand and 8 rows as the columns; its order of k inside a block of
 // 32 is changed so that a lane's four pairs are 16 adjacent bytes, and its order of rows in the second product so that a
-// lane ends up with 8 adjacent outputs of two rows. The inner vectors enter as a high and a low 16-bit part, scaled per row.
+// lane ends up with 8 adjacent outputs of two rows. The inner vectors enter as 16-bit parts, scaled per row, the small parts first.
 #include <mutex>
 #include <string>
 #include <type_traits>
@@ -43,7 +43,7 @@ __device__ __forceinline__ uint4 load16(const void* p, bool take) {
 }
 
 // RT: 16-rank tiles, NT: groups of 8 rows of an item.
-template <int RT, int NT>
+template <typename T, int RT, int NT>
 struct FewCfg {
   static constexpr int kRows = 8 * NT;
   static constexpr int kRanks = RT * 16;
@@ -52,19 +52,20 @@ struct FewCfg {
   static constexpr int kSums = RT * NT <= 8 ? kFewWarps : (RT * NT <= 16 ? 4 : 2);   // places for the warps' sums
   static constexpr int kParts = kSums * kElems * 4;                     // the cluster's sums lie behind them
   static constexpr int kFrag = kParts + kFewCluster * kElems * 4;       // 16-bit parts of the inner vectors, as operands
-  static constexpr int kUp = kFrag + NT * kBlocks * 32 * 32;            // the rows' scales
+  static constexpr int kUp = kFrag + NT * kBlocks * kInnerParts<T> * 32 * 16;   // the rows' scales
   static constexpr int kSmem = kUp + kRows * 4;
   static constexpr int kPerSm = RT * NT == 1 ? 3 : (RT <= 4 ? 2 : 1);
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory");
 };
 
 template <typename T, int RT, int NT>
-__global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_kernel(const __grid_constant__ LoraPass p, int s_log, int parts_log) {
-  using C = FewCfg<RT, NT>;
+__global__ void __launch_bounds__(kFewThreads, FewCfg<T, RT, NT>::kPerSm) lora_few_kernel(const __grid_constant__ LoraPass p, int s_log, int parts_log) {
+  using C = FewCfg<T, RT, NT>;
+  constexpr int kParts = kInnerParts<T>;
   extern __shared__ __align__(16) unsigned char few_smem[];
   float* warp_sum = reinterpret_cast<float*>(few_smem);
   float* part_sum = reinterpret_cast<float*>(few_smem + C::kParts);
-  uint4* frag = reinterpret_cast<uint4*>(few_smem + C::kFrag);          // [group][block][high, low][lane]
+  uint4* frag = reinterpret_cast<uint4*>(few_smem + C::kFrag);          // [group][block][part][lane]
   float* ups = reinterpret_cast<float*>(few_smem + C::kUp);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, s4 = lane & 3;
   const int S = 1 << s_log;                                             // CTAs of a cluster; 1 << parts_log clusters per item
@@ -238,16 +239,12 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_
     if (s4 == 0) ups[n * 8 + g] = up;
 #pragma unroll
     for (int r = 0; r < C::kBlocks; ++r) {
-      uint32_t hi[4], lo[4];
+      uint32_t w[4][kParts];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f0 = v[r][2 * i] * down, f1 = v[r][2 * i + 1] * down;
-        hi[i] = Pair<T>::pack(f0, f1);
-        const float2 w = Pair<T>::unpack(hi[i]);
-        lo[i] = Pair<T>::pack(f0 - w.x, f1 - w.y);
-      }
-      frag[((n * C::kBlocks + r) * 2 + 0) * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      frag[((n * C::kBlocks + r) * 2 + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int i = 0; i < 4; ++i) split<T>(v[r][2 * i] * down, v[r][2 * i + 1] * down, w[i]);
+#pragma unroll
+      for (int q = 0; q < kParts; ++q)
+        frag[((n * C::kBlocks + r) * kParts + q) * 32 + lane] = make_uint4(w[0][q], w[1][q], w[2][q], w[3][q]);
     }
   }
   __syncthreads();
@@ -284,17 +281,17 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[t][i] = 0.f;
 #pragma unroll
-      for (int r = 0; r < C::kBlocks; ++r) {
-        const uint4 hi = frag[((n * C::kBlocks + r) * 2 + 0) * 32 + lane], lo = frag[((n * C::kBlocks + r) * 2 + 1) * 32 + lane];
+      for (int q = kParts - 1; q >= 0; --q)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint4 e = w[r][2 * t], o = w[r][2 * t + 1];
-          mma16816<T>(d[t], e.x, o.x, e.y, o.y, hi.x, hi.y);
-          mma16816<T>(d[t], e.z, o.z, e.w, o.w, hi.z, hi.w);
-          mma16816<T>(d[t], e.x, o.x, e.y, o.y, lo.x, lo.y);
-          mma16816<T>(d[t], e.z, o.z, e.w, o.w, lo.z, lo.w);
+        for (int r = 0; r < C::kBlocks; ++r) {
+          const uint4 h = frag[((n * C::kBlocks + r) * kParts + q) * 32 + lane];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint4 e = w[r][2 * t], o = w[r][2 * t + 1];
+            mma16816<T>(d[t], e.x, o.x, e.y, o.y, h.x, h.y);
+            mma16816<T>(d[t], e.z, o.z, e.w, o.w, h.z, h.w);
+          }
         }
-      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int32_t to = __shfl_sync(0xffffffffu, my_row[n], (2 * s4 + i) * 4);
@@ -314,7 +311,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<RT, NT>::kPerSm) lora_few_
 
 template <typename T, int RT, int NT>
 ks_status_t launch_few(const char* where, const LoraPass& p, cudaStream_t stream) {
-  using C = FewCfg<RT, NT>;
+  using C = FewCfg<T, RT, NT>;
   static std::mutex mu;
   static bool done[64] = {};
   int dev = 0;

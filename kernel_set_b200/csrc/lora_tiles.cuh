@@ -1,6 +1,8 @@
 // Device code shared by the adapters' tensor-core kernels: 16-bit pairs, the scale of an inner vector, and where a tile lies.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "lora_math.cuh"
 
@@ -27,6 +29,23 @@ struct Pair<__nv_bfloat16> {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
 };
+
+// An inner vector is a sum in fp32; it enters the next product as a sum of 16-bit numbers, the first the nearest to it, each further one
+// the nearest to what is left: three of bf16 hold all 24 bits, two of f16 hold 22. (Two of bf16, 2^-18 of the number, changed one in
+// 400 of the outputs in their last place.)
+template <typename T>
+constexpr int kInnerParts = std::is_same<T, __half>::value ? 2 : 3;
+
+template <typename T>
+__device__ __forceinline__ void split(float f0, float f1, uint32_t (&part)[kInnerParts<T>]) {
+#pragma unroll
+  for (int i = 0; i < kInnerParts<T>; ++i) {
+    part[i] = Pair<T>::pack(f0, f1);
+    const float2 w = Pair<T>::unpack(part[i]);
+    f0 -= w.x;
+    f1 -= w.y;
+  }
+}
 
 // The power of two 2^-e for a row whose largest magnitude is `most`, so that most 2^-e is in [1, 2) where possible, and 2^e.
 // It keeps what f16 could not hold (sums beyond 65504, small ones whose low part would vanish) exact; 1 for zeros and non-finite rows.

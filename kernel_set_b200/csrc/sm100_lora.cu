@@ -6,12 +6,13 @@
 // (in rank order, so all CTAs hold the same bits), and each CTA gives its slice of the outputs. The
 // inner vectors never leave the SM, there is one launch, and while the partial sums are exchanged the rows of y0 and V's
 // tiles are already on their way: both phases draw on one ring of shared-memory stages.
-//   warps 0-7   epilogue: two threads per row. Partial sums out of tensor memory, exchange, split into two 16-bit numbers,
+//   warps 0-7   epilogue: two threads per row. Partial sums out of tensor memory, exchange, split into 16-bit parts,
 //               back into tensor memory as the second product's A operand; then y0 + c D, in the stage that holds y0's tile,
 //               and out in 64-byte row segments
 //   warps 8-11  producer: cp.async of 16 bytes. Rows are gathered by number, tails come as zeros, and neither
 //               needs a tensor map (the smallest calls are bound by the host's path)
-//   warp 12     tcgen05.mma: M 128 (rows) x N rank, then M 128 x N 64 (outputs) with K = rank, twice (high and low part)
+//   warp 12     tcgen05.mma: M 128 (rows) x N rank, even and odd chunks into sums of their own (an accumulator is cut off, not rounded,
+//               at each step: 2.1e-6 of the inner vector over 4096 columns in one, 1.0e-6 in two), then M 128 x N 64 (outputs) with K = rank for each part, the small ones first
 // Bound by memory: rows * (d_in + 2 d_out) elements are moved, 2 rank operations for each; the legacy tensor path would be the bound
 // from rank 32 on.
 #include <algorithm>
@@ -45,12 +46,12 @@ struct TileCfg {
   static constexpr int kThreads = (kMmaWarp + 1) * 32;
   static constexpr int kStageBytes = kRowsBytes + RB * kBlockBytes;
   static constexpr int kExchange = kTile * kRanks * 4;
-  static constexpr int kHi = 64 * RB;                  // tensor memory: sums, high part, low part, two output buffers
-  static constexpr int kLo = kHi + 32 * RB;
-  static constexpr int kOut = kLo + 32 * RB;
+  static constexpr int kInner = 2 * kChunk;            // tensor memory: two output buffers, the inner vectors' parts;
+  static constexpr int kInnerCols = 32 * RB;           // the sums lie where the outputs come once they are split
   static constexpr int kTmemCols = RB == 1 ? 256 : 512;
   static constexpr int kPerSm = RB == 1 ? 2 : 1;
-  static_assert(kOut + 2 * kChunk <= kTmemCols, "tensor memory layout");
+  static constexpr int kOdd = RB == 1 ? 64 : 384;      // the sums of the odd chunks
+  static_assert(64 * RB <= kInner && kInner + 3 * kInnerCols <= (RB == 1 ? kTmemCols : kOdd), "tensor memory layout");
   static constexpr int kBars = 3 * kStages + 8;
   static constexpr int kSmem = kStages * kStageBytes + kExchange + kTile * 4 + 8 * kBars + 64;
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory");
@@ -178,7 +179,7 @@ __device__ __forceinline__ void reduce_scatter(uint32_t exchange, int pieces, in
 template <typename T, int RC, bool FWD>
 __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lora_tile_kernel(const __grid_constant__ TileParams q) {
   using C = TileCfg<RC>;
-  constexpr int RB = C::RB;
+  constexpr int RB = C::RB, kParts = kInnerParts<T>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const LoraPass& p = q.p;
   const uint32_t ring = smem_u32(smem);   // (1024-byte aligned: there is no static shared memory)
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
           const uint64_t ad = umma_smem_desc_sw128(a + kk * 32, 16, 1024);
           const uint64_t bd = FWD ? umma_smem_desc_sw128(b + kk * 32, 16, 1024)
                                   : umma_smem_desc_sw128(b + kk * 16 * 128, kBlockBytes, 1024);
-          umma_f16_elect(tmem, ad, bd, q.idesc1, it + kk > 0 ? 1u : 0u);
+          umma_f16_elect(tmem + (it & 1 ? C::kOdd : 0), ad, bd, q.idesc1, it + kk > 1 || kk == 1 ? 1u : 0u);
         }
         tc_commit_elect(free1(s));
       }
@@ -372,13 +373,14 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         fence_async_shared();
         tc_fence_after_sync();
         const uint32_t w = ring + s * C::kStageBytes + kRowsBytes;
-        const uint32_t d = tmem + C::kOut + b * kChunk;
-        for (int kk = 0; kk < q.rank16 / 16; ++kk) {
-          const uint64_t bd = FWD ? umma_smem_desc_sw128(w + (kk >> 2) * kBlockBytes + (kk & 3) * 32, 16, 1024)
-                                  : umma_smem_desc_sw128(w + kk * 16 * 128, kBlockBytes, 1024);
-          umma_f16_tmem_a_elect(d, tmem + C::kHi + kk * 8, bd, q.idesc2, kk > 0 ? 1u : 0u);
-          umma_f16_tmem_a_elect(d, tmem + C::kLo + kk * 8, bd, q.idesc2, 1u);
-        }
+        const uint32_t d = tmem + b * kChunk;
+#pragma unroll
+        for (int part = kParts - 1; part >= 0; --part)
+          for (int kk = 0; kk < q.rank16 / 16; ++kk) {
+            const uint64_t bd = FWD ? umma_smem_desc_sw128(w + (kk >> 2) * kBlockBytes + (kk & 3) * 32, 16, 1024)
+                                    : umma_smem_desc_sw128(w + kk * 16 * 128, kBlockBytes, 1024);
+            umma_f16_tmem_a_elect(d, tmem + C::kInner + part * C::kInnerCols + kk * 8, bd, q.idesc2, part < kParts - 1 || kk > 0 ? 1u : 0u);
+          }
         tc_commit_elect(out_full(b));
       }
     } else {
@@ -393,17 +395,22 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
       joined = true;
       bool ok = n1 == 0 || all_lanes(mbar_wait_long(wctx, bar_sums, 0, 0x37));
       tc_fence_after_sync();
+      const auto own_sums = [&](int b, uint32_t (&x)[16]) {   // 16 ranks of the row, over this CTA's columns
+        tmem_ld(lanes + b * 16, x);
+        tmem_wait_ld(x);
+        if (n1 > 1) {
+          uint32_t odd[16];
+          tmem_ld(lanes + C::kOdd + b * 16, odd);
+          tmem_wait_ld(odd);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(odd[i]));
+        }
+      };
       if (ok && S > 1) {
         // ranks 4 j .. of row r at exchange + (j * 128 + r) * 16
         for (int b = used ? half : blocks; b < blocks; b += 2) {
-          uint32_t x[16];
-          if (n1 > 0) {
-            tmem_ld(lanes + b * 16, x);
-            tmem_wait_ld(x);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = 0u;
-          }
+          uint32_t x[16] = {};
+          if (n1 > 0) own_sums(b, x);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             st_shared_v4(exchange + ((b * 4 + i) * kTile + r) * 16, x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
@@ -434,8 +441,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
               x[4 * i + 3] = v.w;
             }
           } else {
-            tmem_ld(lanes + b * 16, x);
-            tmem_wait_ld(x);
+            own_sums(b, x);
           }
         };
         const int32_t row = row_of[r];
@@ -450,7 +456,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         const float inner_scale = p.scale_inner ? s : 1.f;
         float* inner = p.inner != nullptr && rank == 0 && row >= 0 ? p.inner + static_cast<int64_t>(row) * p.rank : nullptr;
         for (int b = half; b < blocks; b += 2) {
-          uint32_t x[16], hi[8], lo[8];
+          uint32_t x[16], inner_part[kParts][8];
           if (used) {
             sums_of(b, x);
           } else {   // (rows of zeros, whatever tensor memory held)
@@ -467,13 +473,13 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float f0 = __uint_as_float(x[2 * i]) * down, f1 = __uint_as_float(x[2 * i + 1]) * down;
-            hi[i] = Pair<T>::pack(f0, f1);
-            const float2 h = Pair<T>::unpack(hi[i]);
-            lo[i] = Pair<T>::pack(f0 - h.x, f1 - h.y);
+            uint32_t w[kParts];
+            split<T>(__uint_as_float(x[2 * i]) * down, __uint_as_float(x[2 * i + 1]) * down, w);
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) inner_part[part][i] = w[part];
           }
-          tmem_st8(lanes + C::kHi + b * 8, hi);
-          tmem_st8(lanes + C::kLo + b * 8, lo);
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) tmem_st8(lanes + C::kInner + part * C::kInnerCols + b * 8, inner_part[part]);
         }
         tmem_wait_st();
         tc_fence_before_sync();
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
           tc_fence_after_sync();
           if (used) {
             uint32_t d[32];
-            tmem_ld(lanes + C::kOut + b * kChunk + half * 32, d);
+            tmem_ld(lanes + b * kChunk + half * 32, d);
             tmem_wait_ld(d);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -591,37 +597,40 @@ ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, c
 // dA^T [k, rank] = sum over the adapter's rows of x_row g_row^T, and dB [n, rank] = s sum dout_row h_row^T: the same product of a
 // matrix of 16-bit rows, taken in slabs of 256 columns, with fp32 vectors of `rank` numbers. A cluster of CTAs has a slab of one
 // adapter and splits its rows; the parts are added up over distributed shared memory in rank order. Rows are contracted, so both operands
-// are stored with the contracted index outside (MN-major), as they lie in memory; a vector is split into two 16-bit
-// numbers, two MMAs. In f16 the vectors are scaled by a power of two per adapter, from the maxima that the pass before left.
+// are stored with the contracted index outside (MN-major), as they lie in memory; a vector is split into 16-bit
+// parts, the first parts' sums apart from the others', which are small. In f16 the vectors are scaled by a power of two per adapter, from the maxima that the pass before left.
 //   warps 0-7   split vectors (registers, two stages ahead -> shared memory, four warps a stage), at the end the sums
 //   warps 8-11  copies of 64 rows x 512 bytes: one TMA load per 128 bytes of width where the rows lie together (a sequence), cp.async where
 //               they do not (TMA gathers of four rows: 322 us against 196 for 16384 rows of 3 adapters, rank 16: a copy of 512 bytes takes 40 clocks)
-//   warp 12     tcgen05.mma: per stage 2 (128-column halves) x 4 (16 rows each) x 2 (parts), N = rank
+//   warp 12     tcgen05.mma: per stage 2 (128-column halves) x 4 (16 rows each), N = twice the rank (first and second parts side by side, so
+//               that the rows are read once for both), and once more with N = rank for the third parts, added to the second's
 // Bound by memory: every element of x and dout is read once; the vectors are read again from L2 per slab (half the bytes of
 // a slab's rows at rank 64, which is why a slab is as wide as tensor memory and the ring allow two CTAs per SM).
 constexpr int kSlab = 256;
 
-template <int RB>
+template <typename T, int RB>
 struct GradCfg {
-  static constexpr int kStages = RB == 1 ? 2 : 3;
+  static constexpr int kParts = kInnerParts<T>;
+  static constexpr int kStages = RB == 1 || kParts == 3 ? 2 : 3;
   static constexpr int kVecWarps = 8, kMmaWarp = kVecWarps + kProdWarps;
   static constexpr int kThreads = (kMmaWarp + 1) * 32;
   static constexpr int kRows = 64 * kSlab * 2;             // four blocks of 64 rows x 128 bytes
-  static constexpr int kPart = RB * kBlockBytes;           // one 16-bit part of the vectors
-  static constexpr int kStageBytes = kRows + 2 * kPart;
-  static constexpr int kTmemCols = RB == 1 ? 128 : 256;    // two sums of 64 RB columns
+  static constexpr int kPart = RB * kBlockBytes;           // one 16-bit part of the vectors: 64 RB columns
+  static constexpr int kStageBytes = kRows + kParts * kPart;
+  static constexpr int kHalf = 128 * RB;                   // tensor memory of a half: the sums of the first parts and of the others
+  static constexpr int kTmemCols = 2 * kHalf;
   static constexpr int kPerSm = RB == 1 ? 2 : 1;
   static constexpr int kBars = 3 * kStages + 1;
   static constexpr int kSums = kSlab * 64 * RB * 4;        // over the ring, once it is drained
   static_assert(kSums <= kStages * kStageBytes, "the sums lie over the ring");
-  static constexpr int kSmem = 1024 + kStages * kStageBytes + 8 * kBars + 64;
+  static constexpr int kSmem = kStages * kStageBytes + 8 * kBars + 64;
   static_assert(kPerSm * (kSmem + 1024) <= 233472, "shared memory");
 };
 
 struct GradParams {
   LoraWeightGrad p;
   unsigned int* fault_word;
-  uint32_t idesc;
+  uint32_t idesc2, idesc1;   // N = twice the rank, the rank
   int rank16, cluster_log;   // CTAs of a cluster: 1 << cluster_log
   int slabs_a, slabs;     // slabs of x, of both
 };
@@ -658,14 +667,13 @@ __device__ __forceinline__ void add_parts(const LoraWeightGrad& p, uint32_t sums
 }
 
 template <typename T, int RB>
-__global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lora_weight_grad_kernel(const __grid_constant__ GradParams q,
+__global__ void __launch_bounds__(GradCfg<T, RB>::kThreads, GradCfg<T, RB>::kPerSm) lora_weight_grad_kernel(const __grid_constant__ GradParams q,
                                                                                                        const __grid_constant__ CUtensorMap map_x,
                                                                                                        const __grid_constant__ CUtensorMap map_d_out) {
-  using C = GradCfg<RB>;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
+  using C = GradCfg<T, RB>;
+  extern __shared__ __align__(1024) unsigned char smem[];
   const LoraWeightGrad& p = q.p;
-  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const uint32_t ring = smem_u32(smem);
+  const uint32_t ring = smem_u32(smem);   // (1024-byte aligned: there is no static shared memory)
   uint64_t* bar_mem = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes);
   const uint32_t bars = smem_u32(bar_mem);
   const auto full = [&](int s) { return bars + 8u * s; };   // the vectors are there, and rows that were copied one by one
@@ -800,23 +808,22 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
     for (int it = turn; it < n; it += 2) {
       const int s = it % C::kStages;
       if (it >= C::kStages && !(ok = mbar_wait(wctx, freed(s), (it / C::kStages - 1) & 1, 0x42))) break;
-      const uint32_t dst = ring + s * C::kStageBytes + C::kRows + (c8 >> 3) * kBlockBytes;
+      const uint32_t dst = ring + s * C::kStageBytes + C::kRows;
       if (used) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
           const int r = r0 + i * kStep;
           const float f[8] = {v[i][0].x * down, v[i][0].y * down, v[i][0].z * down, v[i][0].w * down,
                               v[i][1].x * down, v[i][1].y * down, v[i][1].z * down, v[i][1].w * down};
-          uint32_t hi[4], lo[4];
+          uint32_t w[4][C::kParts];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            hi[j] = Pair<T>::pack(f[2 * j], f[2 * j + 1]);
-            const float2 h = Pair<T>::unpack(hi[j]);
-            lo[j] = Pair<T>::pack(f[2 * j] - h.x, f[2 * j + 1] - h.y);
+          for (int j = 0; j < 4; ++j) split<T>(f[2 * j], f[2 * j + 1], w[j]);
+          // the first two parts' columns one behind the other, the third in blocks of its own
+#pragma unroll
+          for (int part = 0; part < C::kParts; ++part) {
+            const int c = part < 2 ? part * (q.rank16 / 8) + c8 : 16 * RB + c8;
+            st_shared_v4(dst + (c >> 3) * kBlockBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4), w[0][part], w[1][part], w[2][part], w[3][part]);
           }
-          const uint32_t at = dst + r * 128 + (((c8 & 7) ^ (r & 7)) << 4);
-          st_shared_v4(at, hi[0], hi[1], hi[2], hi[3]);
-          st_shared_v4(at + C::kPart, lo[0], lo[1], lo[2], lo[3]);
         }
       }
       fence_async_shared();
@@ -839,10 +846,10 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           const uint64_t ad = umma_smem_desc_sw128(a + half * 2 * kBlockBytes + kk * 2048, kBlockBytes, 1024);
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-            umma_f16_elect(tmem + half * 64 * RB, ad, umma_smem_desc_sw128(b + part * C::kPart + kk * 2048, kBlockBytes, 1024), q.idesc,
-                           it + kk + part > 0 ? 1u : 0u);
+          umma_f16_elect(tmem + half * C::kHalf, ad, umma_smem_desc_sw128(b + kk * 2048, kBlockBytes, 1024), q.idesc2, it + kk > 0 ? 1u : 0u);
+          if (C::kParts == 3)
+            umma_f16_elect(tmem + half * C::kHalf + q.rank16, ad, umma_smem_desc_sw128(b + 2 * C::kPart + kk * 2048, kBlockBytes, 1024), q.idesc1,
+                           1u);
         }
       }
       tc_commit_elect(freed(s));
@@ -860,19 +867,23 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
   if (warp < C::kVecWarps) {
     tc_fence_after_sync();
     const int half = warp >> 2, col = threadIdx.x & (cols - 1);
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * 64 * RB;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * C::kHalf;
     const uint32_t to = cluster_map_shared(ring + (rank * q.rank16 * cols + col) * 4, threadIdx.x / cols);
     const float c = is_a ? up : up * __ldg(p.scales + adapter);
     for (int b = 0; b < q.rank16 / 16; ++b) {
-      uint32_t x[16];
+      float sum[16] = {};
       if (have) {
+        uint32_t x[16], small[16];
         tmem_ld(lanes + b * 16, x);
+        tmem_ld(lanes + q.rank16 + b * 16, small);
         tmem_wait_ld(x);
+        tmem_wait_ld(small);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[i] = c * (__uint_as_float(x[i]) + __uint_as_float(small[i]));
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (b * 16 + i) * cols * 4), "f"(have ? c * __uint_as_float(x[i]) : 0.f)
-                     : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (b * 16 + i) * cols * 4), "f"(sum[i]) : "memory");
     }
     tc_fence_before_sync();
   }
@@ -890,7 +901,7 @@ __global__ void __launch_bounds__(GradCfg<RB>::kThreads, GradCfg<RB>::kPerSm) lo
 
 template <typename T, int RB>
 ks_status_t launch_grad(const char* where, const GradParams& q, const CUtensorMap (&maps)[2], int64_t items, cudaStream_t stream) {
-  using C = GradCfg<RB>;
+  using C = GradCfg<T, RB>;
   static std::mutex mu;
   static bool done[64] = {};
   int dev = 0;
@@ -953,7 +964,8 @@ ks_status_t lora_weight_grad_pass(const char* where, const LoraWeightGrad& p, ks
   q.fault_word = kernel_fault_word();
   q.rank16 = (p.rank + 15) / 16 * 16;
   const uint32_t fmt = dtype == KS_DTYPE_F16 ? 0u : 1u;
-  q.idesc = umma_instr_desc(fmt, fmt, 1u, 1u, 128u, static_cast<uint32_t>(q.rank16));
+  q.idesc2 = umma_instr_desc(fmt, fmt, 1u, 1u, 128u, static_cast<uint32_t>(2 * q.rank16));
+  q.idesc1 = umma_instr_desc(fmt, fmt, 1u, 1u, 128u, static_cast<uint32_t>(q.rank16));
   q.slabs_a = static_cast<int>((p.k + kSlab - 1) / kSlab);
   q.slabs = q.slabs_a + static_cast<int>((p.n + kSlab - 1) / kSlab);
   const bool wide = p.rank > 64;
