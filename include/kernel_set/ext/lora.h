@@ -48,7 +48,8 @@ KS_API ks_status_t ks_lora_plan(int32_t* sorted_ids, int32_t* offsets,
  * With ks_moe_compute_permutation's offsets and sorted_ids = NULL the rows of a routed
  * layer that are sorted by expert get their expert's adapter.
  * fp32 accumulation, one rounding to `dtype`; A x enters the second product in fp32 or as a sum of 16-bit
- * numbers that hold it to 2^-24 of each element (bf16), 2^-22 (f16). A row whose A x is not finite gets NaN where
+ * numbers that hold it to 2^-24 of each element (bf16), or to 2^-22 of each element and 2^-50 of the row's
+ * largest, whichever is more (f16). A row whose A x is not finite gets NaN where
  * it would get infinities. rank at most 4096.
  */
 KS_API ks_status_t ks_lora_apply(void* out, int64_t ld_out, const void* base,
@@ -74,7 +75,9 @@ KS_API ks_status_t ks_lora_backward_workspace(size_t* bytes, int64_t num_tokens,
  *   d_a, d_b are written whole, with zeros for an adapter without rows
  *   workspace: 16-byte aligned device memory of the size above, undefined on entry and exit; two calls
  *   that may overlap need one each
- * d_out is the gradient of base as it is. Sums in fp32, one rounding; the order of the
+ * d_out is the gradient of base as it is. g and h enter the products as A x does in ks_lora_apply; for d_a and d_b in f16
+ * "largest" is the adapter's, and an adapter whose elements lie further apart than 2^33 (or are not finite) gets plain fp32
+ * sums, slower. Sums in fp32, one rounding; the order of the
  * additions depends on the sizes only.
  */
 KS_API ks_status_t ks_lora_backward(

@@ -123,10 +123,10 @@ ks_status_t check_sizes(const char* where, int64_t rows, int adapters, int rank,
   return KS_SUCCESS;
 }
 
-// The workspace of the backward pass: g [rows, rank], then two maxima per row for f16 (LoraPass).
+// The workspace of the backward pass: g [rows, rank], then two ranges per row for f16 (LoraPass).
 int64_t inner_bytes(int64_t rows, int rank) { return (rows * rank * static_cast<int64_t>(sizeof(float)) + 255) / 256 * 256; }
 int64_t workspace_bytes_of(int64_t rows, int rank) {
-  return inner_bytes(rows, rank) + (2 * rows * static_cast<int64_t>(sizeof(float)) + 255) / 256 * 256;
+  return inner_bytes(rows, rank) + (2 * rows * static_cast<int64_t>(sizeof(float2)) + 255) / 256 * 256;
 }
 
 }  // namespace
@@ -245,8 +245,8 @@ ks_status_t ks_lora_backward(void* d_x, int64_t ld_d_x, void* d_a, void* d_b, co
   const bool tensor = sm100::lora_tile_takes(p) && sm100::lora_weight_grad_takes(w);
   if (tensor && dtype == KS_DTYPE_F16 && num_tokens > 0) {
     p.h = h;
-    w.most_g = p.most_g = reinterpret_cast<float*>(static_cast<char*>(workspace) + inner_bytes(num_tokens, rank));
-    w.most_h = p.most_h = p.most_g + num_tokens;
+    w.range_g = p.range_g = reinterpret_cast<float2*>(static_cast<char*>(workspace) + inner_bytes(num_tokens, rank));
+    w.range_h = p.range_h = p.range_g + num_tokens;
   }
   if (num_tokens > 0) {
     st = run_pass(where, p, false, dtype, s);

@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<T, RT, NT>::kPerSm) lora_f
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     float down, up;
-    row_scale(most, &down, &up);
+    row_scale<T>(most, &down, &up);
     if (s4 == 0) ups[n * 8 + g] = up;
 #pragma unroll
     for (int r = 0; r < C::kBlocks; ++r) {
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<T, RT, NT>::kPerSm) lora_f
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[t][i] = 0.f;
 #pragma unroll
-      for (int q = kParts - 1; q >= 0; --q)
+      for (int q = kParts - 1; q >= 0; --q) {
 #pragma unroll
         for (int r = 0; r < C::kBlocks; ++r) {
           const uint4 h = frag[((n * C::kBlocks + r) * kParts + q) * 32 + lane];
@@ -292,6 +292,13 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<T, RT, NT>::kPerSm) lora_f
             mma16816<T>(d[t], e.z, o.z, e.w, o.w, h.z, h.w);
           }
         }
+        if (kLowUp<T> > 0 && q > 0) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[t][i] *= 1.f / (1 << kLowUp<T>);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int32_t to = __shfl_sync(0xffffffffu, my_row[n], (2 * s4 + i) * 4);

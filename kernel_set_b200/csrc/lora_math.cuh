@@ -18,9 +18,9 @@ struct LoraPass {
   const int32_t* ids;     // may be NULL
   const int32_t* offsets;
   float* inner;           // [rows, rank] fp32, may be NULL: U x (forward), or s U x (backward)
-  const float* h;         // with most_h: [rows, rank] fp32
-  float* most_g;          // may be NULL: [rows] by place; for every 32 places from the start of an adapter's on, at
-  float* most_h;          // the first of them, the largest magnitude of their rows in `inner` and in h
+  const float* h;         // with range_h: [rows, rank] fp32
+  float2* range_g;        // may be NULL: [rows] by place; for every 32 places from the start of an adapter's on, at the first
+  float2* range_h;        // of them, the largest and the smallest magnitude but zero of their rows in `inner` and in h
   int64_t ld_out, ld_base, ld_in;
   int64_t rows;
   int64_t d_in, d_out;
@@ -41,8 +41,8 @@ struct LoraWeightGrad {
   const float* scales;
   const int32_t* ids;
   const int32_t* offsets;
-  const float* most_g;    // as LoraPass's, for f16 on the tensor cores
-  const float* most_h;
+  const float2* range_g;  // as LoraPass's, for f16 on the tensor cores
+  const float2* range_h;
   int64_t ld_x, ld_d_out;
   int64_t rows;
   int64_t k, n;

@@ -32,9 +32,15 @@ struct Pair<__nv_bfloat16> {
 
 // An inner vector is a sum in fp32; it enters the next product as a sum of 16-bit numbers, the first the nearest to it, each further one
 // the nearest to what is left: three of bf16 hold all 24 bits, two of f16 hold 22. (Two of bf16, 2^-18 of the number, changed one in
-// 400 of the outputs in their last place.)
+// 400 of the outputs in their last place.) f16 has few exponents: the vector is scaled (row_scale) so that its largest number is
+// just below 2^15, and the second part is kept 2^kLowUp times as large, its sums brought back behind the product. A number is
+// then held to 2^-22 of itself down to 2^-28 of the largest, and to 2^-50 of the largest below.
 template <typename T>
 constexpr int kInnerParts = std::is_same<T, __half>::value ? 2 : 3;
+template <typename T>
+constexpr int kLowUp = std::is_same<T, __half>::value ? 11 : 0;
+template <typename T>
+constexpr int kTop = std::is_same<T, __half>::value ? 14 : 0;   // exponent of the largest number of a scaled vector
 
 template <typename T>
 __device__ __forceinline__ void split(float f0, float f1, uint32_t (&part)[kInnerParts<T>]) {
@@ -42,20 +48,25 @@ __device__ __forceinline__ void split(float f0, float f1, uint32_t (&part)[kInne
   for (int i = 0; i < kInnerParts<T>; ++i) {
     part[i] = Pair<T>::pack(f0, f1);
     const float2 w = Pair<T>::unpack(part[i]);
-    f0 -= w.x;
-    f1 -= w.y;
+    f0 = (f0 - w.x) * static_cast<float>(1 << kLowUp<T>);
+    f1 = (f1 - w.y) * static_cast<float>(1 << kLowUp<T>);
   }
 }
 
-// The power of two 2^-e for a row whose largest magnitude is `most`, so that most 2^-e is in [1, 2) where possible, and 2^e.
-// It keeps what f16 could not hold (sums beyond 65504, small ones whose low part would vanish) exact; 1 for zeros and non-finite rows.
+// The power of two 2^-e for a vector whose largest magnitude is `most`, so that most 2^-e is in [2^kTop, 2^(kTop+1)) where possible, and 2^e.
+// It keeps what f16 could not hold (sums beyond 65504, small ones whose low part would vanish); 1 for zeros and non-finite vectors.
+template <typename T>
 __device__ __forceinline__ void row_scale(float most, float* down, float* up) {
   uint32_t e = (__float_as_uint(most) >> 23) & 255u;
-  if (e == 0u || e == 255u) e = 127u;
-  e = e > 253u ? 253u : e;
-  *down = __uint_as_float((254u - e) << 23);
-  *up = __uint_as_float(e << 23);
+  if (e == 0u || e == 255u) e = 127u + kTop<T>;
+  e = e > 253u + kTop<T> ? 253u + kTop<T> : e;
+  e = e < kTop<T> + 1u ? kTop<T> + 1u : e;
+  *down = __uint_as_float((254u + kTop<T> - e) << 23);
+  *up = __uint_as_float((e - kTop<T>) << 23);
 }
+
+// How far the numbers of an adapter's vectors lie apart: beyond 2^33 the smallest would be off by more than 2^-17 of themselves.
+__device__ __forceinline__ bool far_apart(float most, float least) { return !(most <= 3.4028234e38f) || least < most * 1.1641532e-10f; }
 
 // Where tile `index` lies: adapter (`adapters` for the rows without one, -1 past the last tile), first place and row count.
 struct TilePlace {

@@ -108,11 +108,15 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-// The largest of the warp's values.
-__device__ __forceinline__ float warp_max(float v) {
+constexpr float kInf = __builtin_huge_valf();
+// The largest of the warp's first values and the smallest of the second.
+__device__ __forceinline__ float2 warp_range(float most, float least) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  for (int o = 16; o > 0; o >>= 1) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  }
+  return make_float2(most, least);
 }
 
 // Whether `ok` (the same for a warp) holds for both warps that share the named barrier `id`. Bounded waits end each on its own, so two
@@ -379,7 +383,9 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
           for (int kk = 0; kk < q.rank16 / 16; ++kk) {
             const uint64_t bd = FWD ? umma_smem_desc_sw128(w + (kk >> 2) * kBlockBytes + (kk & 3) * 32, 16, 1024)
                                     : umma_smem_desc_sw128(w + kk * 16 * 128, kBlockBytes, 1024);
-            umma_f16_tmem_a_elect(d, tmem + C::kInner + part * C::kInnerCols + kk * 8, bd, q.idesc2, part < kParts - 1 || kk > 0 ? 1u : 0u);
+            const uint32_t inner = tmem + C::kInner + part * C::kInnerCols + kk * 8;
+            if (kLowUp<T> > 0 && part == 0 && kk == 0) umma_f16_tmem_a_down_elect<kLowUp<T>>(d, inner, bd, q.idesc2);
+            else umma_f16_tmem_a_elect(d, inner, bd, q.idesc2, part < kParts - 1 || kk > 0 ? 1u : 0u);
           }
         tc_commit_elect(out_full(b));
       }
@@ -445,14 +451,19 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
           }
         };
         const int32_t row = row_of[r];
-        float most = 0.f, down, up;
+        constexpr bool kRanges = std::is_same<T, __half>::value && !FWD;
+        float most = 0.f, least = kInf, down, up;
         for (int b = used ? 0 : blocks; b < blocks; ++b) {
           uint32_t x[16];
           sums_of(b, x);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) most = fmaxf(most, fabsf(__uint_as_float(x[i])));
+          for (int i = 0; i < 16; ++i) {
+            const float v = fabsf(__uint_as_float(x[i]));
+            most = fmaxf(most, v);
+            if (kRanges) least = v > 0.f ? fminf(least, v) : least;
+          }
         }
-        row_scale(most, &down, &up);
+        row_scale<T>(most, &down, &up);
         const float inner_scale = p.scale_inner ? s : 1.f;
         float* inner = p.inner != nullptr && rank == 0 && row >= 0 ? p.inner + static_cast<int64_t>(row) * p.rank : nullptr;
         for (int b = half; b < blocks; b += 2) {
@@ -484,18 +495,23 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
         tmem_wait_st();
         tc_fence_before_sync();
         mbar_arrive(bar_inner);
-        if (p.most_g != nullptr && rank == 0 && half == 0) {
-          float most_h = 0.f;
+        if (kRanges && p.range_g != nullptr && rank == 0 && half == 0) {
+          float most_h = 0.f, least_h = kInf;
           if (row >= 0)
             for (int i = 0; i < p.rank; i += 4) {
               const float4 v = __ldg(reinterpret_cast<const float4*>(p.h + static_cast<int64_t>(row) * p.rank + i));
-              most_h = fmaxf(fmaxf(fmaxf(most_h, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
+              const float f[4] = {fabsf(v.x), fabsf(v.y), fabsf(v.z), fabsf(v.w)};
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                most_h = fmaxf(most_h, f[u]);
+                least_h = f[u] > 0.f ? fminf(least_h, f[u]) : least_h;
+              }
             }
-          most_h = warp_max(most_h);
-          const float most_g = warp_max(row >= 0 ? most * fabsf(inner_scale) : 0.f);
+          const float2 range_g = warp_range(row >= 0 ? most * fabsf(inner_scale) : 0.f, row >= 0 ? least * fabsf(inner_scale) : kInf);
+          const float2 range_h = warp_range(most_h, least_h);
           if (lane == 0 && quarter * 32 < count) {
-            p.most_g[place + quarter * 32] = most_g;
-            p.most_h[place + quarter * 32] = most_h;
+            p.range_g[place + quarter * 32] = range_g;
+            p.range_h[place + quarter * 32] = range_h;
           }
         }
         // second product: y0 + c D in the stage that holds y0, then out: of the quarter's 32 rows a warp stores 16, 128 bytes of each
@@ -598,7 +614,8 @@ ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, c
 // matrix of 16-bit rows, taken in slabs of 256 columns, with fp32 vectors of `rank` numbers. A cluster of CTAs has a slab of one
 // adapter and splits its rows; the parts are added up over distributed shared memory in rank order. Rows are contracted, so both operands
 // are stored with the contracted index outside (MN-major), as they lie in memory; a vector is split into 16-bit
-// parts, the first parts' sums apart from the others', which are small. In f16 the vectors are scaled by a power of two per adapter, from the maxima that the pass before left.
+// parts, the first parts' sums apart from the others', which are small. In f16 the vectors are scaled by a power of two per adapter, from the ranges that the pass before left; where an adapter's numbers lie
+// further apart than the parts can hold (a factor of 2^33) its sums are made once more in fp32, row by row.
 //   warps 0-7   split vectors (registers, two stages ahead -> shared memory, four warps a stage), at the end the sums
 //   warps 8-11  copies of 64 rows x 512 bytes: one TMA load per 128 bytes of width where the rows lie together (a sequence), cp.async where
 //               they do not (TMA gathers of four rows: 322 us against 196 for 16384 rows of 3 adapters, rank 16: a copy of 512 bytes takes 40 clocks)
@@ -666,6 +683,33 @@ __device__ __forceinline__ void add_parts(const LoraWeightGrad& p, uint32_t sums
   }
 }
 
+// The sums of the places [first, last) for a column and the ranks j .. j + 15, in fp32, row by row.
+template <typename T>
+__device__ __forceinline__ void plain_sums(float (&sum)[16], const LoraWeightGrad& p, bool is_a, int64_t first, int64_t last, int64_t col, int j,
+                                        float scale) {
+  const T* m = static_cast<const T*>(is_a ? p.x : p.d_out) + col;
+  const int64_t ld = is_a ? p.ld_x : p.ld_d_out;
+  const float* vecs = (is_a ? p.g : p.h) + j;
+  float acc[16] = {};
+#pragma unroll 1
+  for (int64_t place = first; place < last; ++place) {
+    const int64_t row = lora_row(p.ids, place, p.rows);
+    if (row < 0) continue;
+    const float x = to_f32<T>(m[row * ld]);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      if (j + i >= p.rank) continue;
+      const float4 v = __ldg(reinterpret_cast<const float4*>(vecs + row * p.rank + i));
+      acc[i] = fmaf(v.x, x, acc[i]);
+      acc[i + 1] = fmaf(v.y, x, acc[i + 1]);
+      acc[i + 2] = fmaf(v.z, x, acc[i + 2]);
+      acc[i + 3] = fmaf(v.w, x, acc[i + 3]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum[i] = scale * acc[i];
+}
+
 template <typename T, int RB>
 __global__ void __launch_bounds__(GradCfg<T, RB>::kThreads, GradCfg<T, RB>::kPerSm) lora_weight_grad_kernel(const __grid_constant__ GradParams q,
                                                                                                        const __grid_constant__ CUtensorMap map_x,
@@ -722,6 +766,7 @@ __global__ void __launch_bounds__(GradCfg<T, RB>::kThreads, GradCfg<T, RB>::kPer
     return at < count ? static_cast<int32_t>(lora_row(p.ids, begin + at, p.rows)) : -1;
   };
   float up = 1.f;
+  bool far = false;
 
   if (warp >= C::kVecWarps && warp < C::kMmaWarp) {
     // ---- copies. 64 rows that lie together come by TMA; others one by one: a warp takes every fourth, a lane 16 bytes of it ----
@@ -778,10 +823,15 @@ __global__ void __launch_bounds__(GradCfg<T, RB>::kThreads, GradCfg<T, RB>::kPer
     const bool used = c8 * 8 < q.rank16, has = c8 * 8 < p.rank;
     float down = 1.f;
     if (std::is_same<T, __half>::value) {
-      const float* most = is_a ? p.most_g : p.most_h;
-      float m = 0.f;
-      for (int64_t i = lane; i * 32 < count; i += 32) m = fmaxf(m, __ldg(most + begin + i * 32));
-      row_scale(warp_max(m), &down, &up);
+      const float2* ranges = is_a ? p.range_g : p.range_h;
+      float2 r = make_float2(0.f, kInf);
+      for (int64_t i = lane; i * 32 < count; i += 32) {
+        const float2 v = __ldg(ranges + begin + i * 32);
+        r = make_float2(fmaxf(r.x, v.x), fminf(r.y, v.y));
+      }
+      r = warp_range(r.x, r.y);
+      row_scale<T>(r.x, &down, &up);
+      far = far_apart(r.x, r.y);
     }
     int32_t row[kMine];
     float4 v[kMine][2];
@@ -869,7 +919,7 @@ __global__ void __launch_bounds__(GradCfg<T, RB>::kThreads, GradCfg<T, RB>::kPer
     const int half = warp >> 2, col = threadIdx.x & (cols - 1);
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * C::kHalf;
     const uint32_t to = cluster_map_shared(ring + (rank * q.rank16 * cols + col) * 4, threadIdx.x / cols);
-    const float c = is_a ? up : up * __ldg(p.scales + adapter);
+    const float scale = is_a ? 1.f : __ldg(p.scales + adapter), c = scale * up;
     for (int b = 0; b < q.rank16 / 16; ++b) {
       float sum[16] = {};
       if (have) {
@@ -879,7 +929,11 @@ __global__ void __launch_bounds__(GradCfg<T, RB>::kThreads, GradCfg<T, RB>::kPer
         tmem_wait_ld(x);
         tmem_wait_ld(small);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum[i] = c * (__uint_as_float(x[i]) + __uint_as_float(small[i]));
+        for (int i = 0; i < 16; ++i) sum[i] = c * fmaf(__uint_as_float(small[i]), 1.f / (1 << kLowUp<T>), __uint_as_float(x[i]));
+        if (far && col0 + threadIdx.x < width) {
+          plain_sums<T>(sum, p, is_a, begin + chunk0 * 64, begin + min(count, (chunk0 + n) * 64), col0 + threadIdx.x, b * 16, scale);
+        }
+        __syncwarp();
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i)

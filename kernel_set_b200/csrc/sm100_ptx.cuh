@@ -471,6 +471,15 @@ __device__ __forceinline__ void umma_f16_tmem_a_elect(uint32_t d_tmem, uint32_t 
                "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
                : "memory");
 }
+// Same, on top of what D holds times 2^-DOWN.
+template <int DOWN>
+__device__ __forceinline__ void umma_f16_tmem_a_down_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc) {
+  asm volatile("{\n\t.reg .pred p;\n\t" KSB_ELECT_PROLOGUE
+               "setp.eq.b32 p, 0, 0;\n\t"
+               "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, %4;\n\t}\n" ::"r"(d_tmem),
+               "r"(a_tmem), "l"(b_desc), "r"(idesc), "n"(DOWN)
+               : "memory");
+}
 __device__ __forceinline__ void tc_commit_elect(uint32_t bar) {
   asm volatile("{\n\t" KSB_ELECT_PROLOGUE
                "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar)

@@ -5,7 +5,7 @@ out. The tests build inner numbers of which all but the last bits cancel."""
 import pytest
 import torch
 
-from _lora import STEP, half_step
+from _lora import STEP, Problem, chain, check, half_step
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +87,80 @@ def test_factors_gradients_see_all_bits_of_the_inner_vectors(ks, cuda, adapters,
     h[::2], h[1::2] = v[:, None], (first + second)[:, None]
     _, _, d_b = call(signs.expand(-1, n), base, h)
     _expect("d_b", d_b, last[:, None, None].expand(-1, n, rank), first[:, None, None])
+
+
+def _falling(rank, size, device):
+    """Factors 1 .. size over the ranks, powers of two."""
+    return torch.exp2(torch.round(torch.linspace(0, size, rank, device=device)))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rank", [8, 24, 64, 128])
+@pytest.mark.parametrize("tokens", [3, 40, 700])
+def test_outputs_of_ranks_far_below_the_largest(ks, cuda, tokens, rank, dtype):
+    """The numbers of an inner vector fall to 2^-18 of the largest (which f16 factors can express), and every output depends on one of them."""
+    p = Problem(tokens, 2, rank, 64, 128, dtype, seed=rank)
+    fall = _falling(rank, -18, cuda)
+    owner = torch.arange(128, device=cuda) % rank
+    mask = owner[:, None] == torch.arange(rank, device=cuda)
+    ids, offsets = ks.lora.plan(p.ids, p.adapters)
+    p.a = (p.a.float() * fall[:, None]).to(dtype)
+    p.b = torch.where(mask, p.b.float() / fall * 2.0 ** -8, 0).to(dtype)
+    p.base = torch.zeros_like(p.base)
+    want, bound, _, _ = p.forward()
+    out = ks.lora.apply(torch.empty_like(p.base), p.base, p.x, p.a, p.b, p.scales, ids, offsets)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    check("out", out, want, bound + tiny)
+    # the roles of the factors changed: g falls, and every column of d_x depends on one of its numbers
+    p = Problem(tokens, 2, rank, 128, 64, dtype, seed=rank)
+    p.b = (p.b.float() * fall).to(dtype)
+    p.a = torch.where(mask.t(), p.a.float() / fall[:, None] * 2.0 ** -4, 0).to(dtype).contiguous()
+    p.d_x_base = torch.zeros_like(p.d_x_base)
+    h = torch.zeros(tokens, rank, device=cuda)
+    want, bounds = p.backward(h)
+    got = ks.lora.backward(torch.empty_like(p.x), torch.empty_like(p.a), torch.empty_like(p.b), p.d_x_base, p.d_out, p.x, h, p.a, p.b, p.scales,
+                           ids, offsets)
+    check("d_x", got[0], want[0], bounds[0])
+    check("d_a", got[1], want[1], bounds[1])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rank", [8, 64, 128])
+@pytest.mark.parametrize("fall", [-14, -20, -30, -45, -90])
+@pytest.mark.parametrize("tokens", [70, 1500])
+def test_gradients_of_ranks_far_below_the_largest(ks, cuda, tokens, fall, rank, dtype):
+    """h falls over the ranks, and each of d_b's elements is held to its own sum."""
+    p = Problem(tokens, 2, rank, 72, 264, dtype, seed=tokens)
+    ids, offsets = ks.lora.plan(p.ids, p.adapters)
+    g = torch.Generator(device=cuda).manual_seed(rank)
+    h = torch.randn(tokens, rank, generator=g, device=cuda) * _falling(rank, fall, cuda) * 2.0 ** 12
+    want, bounds = p.backward(h)
+    got = ks.lora.backward(torch.empty_like(p.x), torch.empty_like(p.a), torch.empty_like(p.b), p.d_x_base, p.d_out, p.x, h, p.a, p.b, p.scales,
+                           ids, offsets)
+    for what, x, y, b in zip(("d_x", "d_a", "d_b"), got, want, bounds):
+        check(what, x, y, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rank", [16, 96])
+@pytest.mark.parametrize("size", [12, 24, 34, 60, 100])
+@pytest.mark.parametrize("tokens", [70, 1500])
+def test_gradients_beside_a_row_far_above_the_others(ks, cuda, tokens, size, rank, dtype):
+    """A row whose h is huge and whose d_out is zero, and one whose g is large and whose x is zero, change nothing."""
+    p = Problem(tokens, 2, rank, 264, 136, dtype, seed=tokens + 1)
+    ids, offsets = ks.lora.plan(p.ids, p.adapters)
+    g = torch.Generator(device=cuda).manual_seed(rank)
+    h = torch.randn(tokens, rank, generator=g, device=cuda)
+    h[tokens // 2] *= 2.0 ** size
+    p.d_out[tokens // 2] = 0
+    top = 13 if dtype is HF else size
+    p.d_out[tokens // 3] *= 2.0 ** top
+    p.d_out[[i for i in range(tokens) if i != tokens // 3]] *= 2.0 ** (top - size if dtype is HF and size <= 24 else 0)
+    p.x[tokens // 3] = 0
+    p.b = (p.b.float() * 2.0 ** -6).to(dtype)
+    h[tokens // 3] = 0
+    want, bounds = p.backward(h)
+    got = ks.lora.backward(torch.empty_like(p.x), torch.empty_like(p.a), torch.empty_like(p.b), p.d_x_base, p.d_out, p.x, h, p.a, p.b, p.scales,
+                           ids, offsets)
+    for what, x, y, b in zip(("d_a", "d_b"), got[1:], want[1:], bounds[1:]):
+        check(what, x, y, b)
