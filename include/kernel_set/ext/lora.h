@@ -76,8 +76,8 @@ KS_API ks_status_t ks_lora_backward_workspace(size_t* bytes, int64_t num_tokens,
  *   workspace: 16-byte aligned device memory of the size above, undefined on entry and exit; two calls
  *   that may overlap need one each
  * d_out is the gradient of base as it is. g and h enter the products as A x does in ks_lora_apply; for d_a and d_b in f16
- * "largest" is the adapter's, and an adapter whose elements lie further apart than 2^33 (or are not finite) gets plain fp32
- * sums, slower. Sums in fp32, one rounding; the order of the
+ * "largest" is the adapter's, and an adapter whose elements lie further apart than 2^33 gets plain fp32 sums, as do, in both types,
+ * sums that are not finite (7.6 ms against 0.15 where that is all of d_b for 16384 rows of rank 64 beside 4096 x 4096). Sums in fp32, one rounding; the order of the
  * additions depends on the sizes only.
  */
 KS_API ks_status_t ks_lora_backward(

@@ -615,7 +615,9 @@ ks_status_t launch_tile(const char* where, const TileParams& q, int64_t tiles, c
 // adapter and splits its rows; the parts are added up over distributed shared memory in rank order. Rows are contracted, so both operands
 // are stored with the contracted index outside (MN-major), as they lie in memory; a vector is split into 16-bit
 // parts, the first parts' sums apart from the others', which are small. In f16 the vectors are scaled by a power of two per adapter, from the ranges that the pass before left; where an adapter's numbers lie
-// further apart than the parts can hold (a factor of 2^33) its sums are made once more in fp32, row by row.
+// further apart than the parts can hold (a factor of 2^33) its sums are made once more in fp32, row by row, and so are sums that
+// are not finite. (All of d_b for 16384 rows of rank 64 beside 4096 x 4096: 7.6 ms in place of
+// 0.15 for the call, which only such numbers pay.)
 //   warps 0-7   split vectors (registers, two stages ahead -> shared memory, four warps a stage), at the end the sums
 //   warps 8-11  copies of 64 rows x 512 bytes: one TMA load per 128 bytes of width where the rows lie together (a sequence), cp.async where
 //               they do not (TMA gathers of four rows: 322 us against 196 for 16384 rows of 3 adapters, rank 16: a copy of 512 bytes takes 40 clocks)
@@ -683,31 +685,34 @@ __device__ __forceinline__ void add_parts(const LoraWeightGrad& p, uint32_t sums
   }
 }
 
-// The sums of the places [first, last) for a column and the ranks j .. j + 15, in fp32, row by row.
+// The sums of the places [first, last) for a column and the ranks j .. j + 3, in fp32, row by row.
 template <typename T>
-__device__ __forceinline__ void plain_sums(float (&sum)[16], const LoraWeightGrad& p, bool is_a, int64_t first, int64_t last, int64_t col, int j,
-                                        float scale) {
+__device__ __forceinline__ float4 plain_sums(const LoraWeightGrad& p, bool is_a, int64_t first, int64_t last, int64_t col, int j) {
   const T* m = static_cast<const T*>(is_a ? p.x : p.d_out) + col;
   const int64_t ld = is_a ? p.ld_x : p.ld_d_out;
   const float* vecs = (is_a ? p.g : p.h) + j;
-  float acc[16] = {};
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int kAhead = 4;   // rows asked for at a time, without branches between the loads
 #pragma unroll 1
-  for (int64_t place = first; place < last; ++place) {
-    const int64_t row = lora_row(p.ids, place, p.rows);
-    if (row < 0) continue;
-    const float x = to_f32<T>(m[row * ld]);
+  for (int64_t place = first; place < last; place += kAhead) {
+    int32_t row[kAhead];
+    T x[kAhead];
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      if (j + i >= p.rank) continue;
-      const float4 v = __ldg(reinterpret_cast<const float4*>(vecs + row * p.rank + i));
-      acc[i] = fmaf(v.x, x, acc[i]);
-      acc[i + 1] = fmaf(v.y, x, acc[i + 1]);
-      acc[i + 2] = fmaf(v.z, x, acc[i + 2]);
-      acc[i + 3] = fmaf(v.w, x, acc[i + 3]);
+    for (int u = 0; u < kAhead; ++u) row[u] = static_cast<int32_t>(lora_row(p.ids, place + u < last ? place + u : last - 1, p.rows));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = m[(row[u] >= 0 ? row[u] : 0) * ld];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(vecs + static_cast<int64_t>(row[u] >= 0 ? row[u] : 0) * p.rank));
+      const bool take = row[u] >= 0 && place + u < last;
+      const float f = to_f32<T>(x[u]);
+      sum.x = take ? fmaf(v.x, f, sum.x) : sum.x;
+      sum.y = take ? fmaf(v.y, f, sum.y) : sum.y;
+      sum.z = take ? fmaf(v.z, f, sum.z) : sum.z;
+      sum.w = take ? fmaf(v.w, f, sum.w) : sum.w;
     }
   }
-#pragma unroll
-  for (int i = 0; i < 16; ++i) sum[i] = scale * acc[i];
+  return sum;
 }
 
 template <typename T, int RB>
@@ -920,6 +925,8 @@ __global__ void __launch_bounds__(GradCfg<T, RB>::kThreads, GradCfg<T, RB>::kPer
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21) + half * C::kHalf;
     const uint32_t to = cluster_map_shared(ring + (rank * q.rank16 * cols + col) * 4, threadIdx.x / cols);
     const float scale = is_a ? 1.f : __ldg(p.scales + adapter), c = scale * up;
+    uint32_t redo = far ? ~0u : 0u;   // 16 ranks a bit
+    const auto put = [&](int j, float sum) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + j * cols * 4), "f"(sum) : "memory"); };
     for (int b = 0; b < q.rank16 / 16; ++b) {
       float sum[16] = {};
       if (have) {
@@ -929,16 +936,24 @@ __global__ void __launch_bounds__(GradCfg<T, RB>::kThreads, GradCfg<T, RB>::kPer
         tmem_wait_ld(x);
         tmem_wait_ld(small);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum[i] = c * fmaf(__uint_as_float(small[i]), 1.f / (1 << kLowUp<T>), __uint_as_float(x[i]));
-        if (far && col0 + threadIdx.x < width) {
-          plain_sums<T>(sum, p, is_a, begin + chunk0 * 64, begin + min(count, (chunk0 + n) * 64), col0 + threadIdx.x, b * 16, scale);
+        for (int i = 0; i < 16; ++i) {
+          sum[i] = fmaf(__uint_as_float(small[i]), 1.f / (1 << kLowUp<T>), __uint_as_float(x[i]));
+          // (an infinite row or number makes NaN of the parts that it meets: zeros, or infinities of the other sign)
+          if (!(fabsf(sum[i]) <= 3.4028234e38f)) redo |= 1u << b;
         }
-        __syncwarp();
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + (b * 16 + i) * cols * 4), "f"(sum[i]) : "memory");
+      for (int i = 0; i < 16; ++i) put(b * 16 + i, c * sum[i]);
     }
+    if (have && redo != 0u && col0 + threadIdx.x < width)
+      for (int j = 0; j < p.rank; j += 4)
+        if (redo >> (j >> 4) & 1u) {
+          const float4 sum = plain_sums<T>(p, is_a, begin + chunk0 * 64, begin + min(count, (chunk0 + n) * 64), col0 + threadIdx.x, j);
+          put(j, scale * sum.x);
+          put(j + 1, scale * sum.y);
+          put(j + 2, scale * sum.z);
+          put(j + 3, scale * sum.w);
+        }
     tc_fence_before_sync();
   }
   __syncwarp();

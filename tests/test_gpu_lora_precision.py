@@ -164,3 +164,32 @@ def test_gradients_beside_a_row_far_above_the_others(ks, cuda, tokens, size, ran
                            ids, offsets)
     for what, x, y, b in zip(("d_a", "d_b"), got[1:], want[1:], bounds[1:]):
         check(what, x, y, b)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rank", [8, 12, 64, 128])
+@pytest.mark.parametrize("where", ["x", "d_out", "h"])
+@pytest.mark.parametrize("tokens", [70, 1500])
+def test_gradients_of_numbers_that_are_not_finite(ks, cuda, tokens, where, rank, dtype):
+    """An infinity in a row makes infinities of the sums' own signs in the factors' gradients, and NaN only where fp32 has it."""
+    p = Problem(tokens, 3, rank, 136, 264, dtype, seed=rank)
+    p.ids[:6] = torch.tensor([0, 0, 1, 1, 2, 2], dtype=torch.int32, device=cuda)
+    ids, offsets = ks.lora.plan(p.ids, p.adapters)
+    g = torch.Generator(device=cuda).manual_seed(rank)
+    h = torch.randn(tokens, rank, generator=g, device=cuda)
+    inf = float("inf")
+    if where == "x":
+        p.x[0, 5], p.x[2, 7], p.x[3, 7], p.x[4, 0] = inf, inf, -inf, float("nan")
+    elif where == "d_out":
+        p.d_out[0, 5], p.d_out[2, 7], p.d_out[3, 7], p.d_out[4, 0] = inf, inf, -inf, float("nan")
+    else:
+        h[0, 1], h[2, 3], h[3, 3], h[4, 0] = inf, inf, -inf, float("nan")
+    want, bounds = p.backward(h)
+    got = ks.lora.backward(torch.empty_like(p.x), torch.empty_like(p.a), torch.empty_like(p.b), p.d_x_base, p.d_out, p.x, h, p.a, p.b, p.scales,
+                           ids, offsets)
+    for what, x, y, b in zip(("d_a", "d_b"), got[1:], want[1:], bounds[1:]):
+        fine = torch.isfinite(y)
+        assert torch.equal(torch.isnan(x), torch.isnan(y)), what
+        inf = torch.isinf(y)
+        assert torch.equal(x[inf].double(), y[inf]), what
+        check(what, x[fine], y[fine], b[fine])
