@@ -27,8 +27,9 @@ def plan(adapter_ids: torch.Tensor, num_adapters: int, sorted_ids: Optional[torc
          offsets: Optional[torch.Tensor] = None, stream: TensorLike = None):
     """The rows sorted by adapter. ``adapter_ids [tokens]`` int32, an id outside ``[0, num_adapters)`` stands for
     "none". Returns ``(sorted_ids [tokens], offsets [num_adapters + 2])``, both int32, in the given buffers if any."""
-    if adapter_ids.dtype != torch.int32:
-        raise ValueError(f"adapter_ids must be int32; got {adapter_ids.dtype}")
+    for name, given in (("adapter_ids", adapter_ids), ("sorted_ids", sorted_ids), ("offsets", offsets)):
+        if given is not None and given.dtype != torch.int32:
+            raise ValueError(f"{name} must be int32; got {given.dtype}")
     tokens = adapter_ids.numel()
     if sorted_ids is None:
         sorted_ids = torch.empty(tokens, dtype=torch.int32, device=adapter_ids.device)

@@ -135,3 +135,17 @@ def test_moe_backward_wrappers_refuse(ks):
         for b in bad:
             with pytest.raises(ValueError, match="must be torch|elements where"):
                 fn(**{**good, **b})
+
+
+def test_plan_refuses_buffers_of_other_types_and_sizes(ks):
+    """They are written as int32: 64-bit ones have the right count and would hold pairs of numbers."""
+    ids = torch.zeros(6, dtype=torch.int32)
+    for sorted_ids, offsets, what in ((torch.zeros(6, dtype=torch.int64), None, "sorted_ids must be int32"),
+                                      (None, torch.zeros(4, dtype=torch.int64), "offsets must be int32"),
+                                      (torch.zeros(6), None, "sorted_ids must be int32"),
+                                      (torch.zeros(5, dtype=torch.int32), None, "expected"),
+                                      (None, torch.zeros(5, dtype=torch.int32), "expected")):
+        with pytest.raises(ValueError, match=what):
+            ks.lora.plan(ids, 2, sorted_ids, offsets)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        ks.lora.plan(ids, 2, torch.zeros(6, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
