@@ -122,6 +122,16 @@ def on_device_of(obj: TensorLike):
     return _HERE
 
 
+def allocating_on(stream: TensorLike, device: torch.device):
+    """A context in which torch allocates from the pool of ``stream`` (``None``: of the current stream, as ever). What a call gives to
+    kernels on ``stream`` comes from there: a block of another stream's pool may still be in use by that stream's kernels, behind which
+    nothing orders ``stream``."""
+    if stream is None or device.type != "cuda":
+        return _HERE
+    handle = stream_ptr(stream)   # (ExternalStream(0) would be a new stream)
+    return torch.cuda.stream(torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device))
+
+
 def same_dtype(reference: TensorLike, **others: TensorLike) -> None:
     """Refuses tensors whose type is not ``reference``'s (raw addresses have none)."""
     if isinstance(reference, torch.Tensor):

@@ -20,21 +20,24 @@ from typing import Optional
 import torch
 
 from ._lib import by_address as lib, check
-from ._tensor import TensorLike, default_stream, dtype_to_ks, i32_ptr, on_device_of, ptr, stream_ptr
+from ._tensor import TensorLike, allocating_on, default_stream, dtype_to_ks, i32_ptr, on_device_of, ptr
 
 
 def plan(adapter_ids: torch.Tensor, num_adapters: int, sorted_ids: Optional[torch.Tensor] = None,
          offsets: Optional[torch.Tensor] = None, stream: TensorLike = None):
     """The rows sorted by adapter. ``adapter_ids [tokens]`` int32, an id outside ``[0, num_adapters)`` stands for
-    "none". Returns ``(sorted_ids [tokens], offsets [num_adapters + 2])``, both int32, in the given buffers if any."""
+    "none". Returns ``(sorted_ids [tokens], offsets [num_adapters + 2])``, both int32, in the given buffers if any. With ``stream``,
+    buffers that it makes belong to that stream, as if they had been made with it as the current one."""
     for name, given in (("adapter_ids", adapter_ids), ("sorted_ids", sorted_ids), ("offsets", offsets)):
         if given is not None and given.dtype != torch.int32:
             raise ValueError(f"{name} must be int32; got {given.dtype}")
     tokens = adapter_ids.numel()
-    if sorted_ids is None:
-        sorted_ids = torch.empty(tokens, dtype=torch.int32, device=adapter_ids.device)
-    if offsets is None:
-        offsets = torch.empty(int(num_adapters) + 2, dtype=torch.int32, device=adapter_ids.device)
+    if sorted_ids is None or offsets is None:
+        with allocating_on(stream, adapter_ids.device):
+            if sorted_ids is None:
+                sorted_ids = torch.empty(tokens, dtype=torch.int32, device=adapter_ids.device)
+            if offsets is None:
+                offsets = torch.empty(int(num_adapters) + 2, dtype=torch.int32, device=adapter_ids.device)
     _sizes(num_adapters=(offsets.numel(), int(num_adapters) + 2), tokens=(sorted_ids.numel(), tokens))
     with on_device_of(adapter_ids):
         check(lib.ks_lora_plan(i32_ptr(sorted_ids, name="sorted_ids"), i32_ptr(offsets, name="offsets"),
@@ -140,7 +143,8 @@ def backward(d_x: torch.Tensor, d_a: torch.Tensor, d_b: torch.Tensor, d_x_base: 
     """Gradient of :func:`apply`: with ``g = s B^T d_out`` per row, ``d_x = d_x_base + A^T g`` (``d_x`` may be
     ``d_x_base``, the gradient through the shared projection), ``d_a = sum g x^T`` and ``d_b = s sum d_out h^T`` over each
     adapter's rows, zeros for an adapter without rows. ``h`` is what the forward pass kept. ``d_out`` is the gradient of
-    ``base`` as it is. Types and shapes as in :func:`apply`; ``workspace``: uint8, allocated if not given.
+    ``base`` as it is. Types and shapes as in :func:`apply`; ``workspace``: uint8, allocated (from
+    ``stream``'s pool) if not given.
     Returns ``(d_x, d_a, d_b)``."""
     tokens, k, adapters, n, rank = _dims(x, b)
     dt = x.dtype
@@ -162,9 +166,8 @@ def backward(d_x: torch.Tensor, d_a: torch.Tensor, d_b: torch.Tensor, d_x_base: 
         _refuse({"d_x": (d_x, (tokens, k), dt), "d_x_base": (d_x_base, (tokens, k), dt), "d_out": (d_out, (tokens, n), dt),
                  "x": (x, (tokens, k), dt)}, flat, sorted_ids, offsets, adapters)
     if workspace is None:
-        workspace = torch.empty(backward_workspace(tokens, adapters, rank, k, n), dtype=torch.uint8, device=x.device)
-        if stream is not None:   # it goes back to its pool when this returns
-            workspace.record_stream(torch.cuda.ExternalStream(stream_ptr(stream), device=x.device))
+        with allocating_on(stream, x.device):   # (it goes back to that stream's pool when this returns: later calls there come behind)
+            workspace = torch.empty(backward_workspace(tokens, adapters, rank, k, n), dtype=torch.uint8, device=x.device)
     with on_device_of(x):
         check(lib.ks_lora_backward(d_x.data_ptr(), ld_d_x, d_a.data_ptr(), d_b.data_ptr(), d_x_base.data_ptr(), ld_d_x_base,
                                    d_out.data_ptr(), ld_d_out, x.data_ptr(), ld_x, h.data_ptr(), a.data_ptr(), b.data_ptr(),
