@@ -43,8 +43,9 @@ KS_API ks_status_t ks_lora_plan(int32_t* sorted_ids, int32_t* offsets,
  *   sorted_ids   as ks_lora_plan gives them, or NULL: row i is at place i. Places with an
  *                id outside [0, num_tokens) are left out, and a row whose id is at no place
  *                is left as it was; a row may be at one place
- *   offsets      [num_adapters + 1]: places offsets[a] .. offsets[a+1] have adapter a, places from
- *                offsets[num_adapters] on none. Values are clamped to [0, num_tokens].
+ *   offsets      [num_adapters + 1], ascending: places offsets[a] .. offsets[a+1] have adapter a, places from
+ *                offsets[num_adapters] on none; places in front of offsets[0] are left out (part of a longer
+ *                table, as a rank's own experts'). Values are clamped to [0, num_tokens].
  * With ks_moe_compute_permutation's offsets and sorted_ids = NULL the rows of a routed
  * layer that are sorted by expert get their expert's adapter.
  * fp32 accumulation, one rounding to `dtype`; A x enters the second product in fp32 or as a sum of 16-bit

@@ -33,6 +33,7 @@ __global__ void __launch_bounds__(kAnyThreads) lora_any_kernel(LoraPass p) {
   const int64_t row = lora_row(p.ids, place, p.rows);
   if (row < 0) return;
   const int a = lora_adapter(p.offsets, p.adapters, place, p.rows);
+  if (a < 0) return;
   const T* base = static_cast<const T*>(p.base) + row * p.ld_base;
   T* out = static_cast<T*>(p.out) + row * p.ld_out;
   if (a >= p.adapters) {

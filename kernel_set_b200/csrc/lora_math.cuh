@@ -60,9 +60,9 @@ __device__ __forceinline__ int64_t lora_offset(const int32_t* __restrict__ offse
   const int64_t o = __ldg(offsets + a);
   return o < 0 ? 0 : (o > rows ? rows : o);
 }
-// The adapter of place p: the last a with offsets[a] <= p, `adapters` when p lies behind the last one's rows.
+// The adapter of place p: the last a with offsets[a] <= p, `adapters` when p lies behind the last one's rows, -1 in front of the first's.
 __device__ __forceinline__ int lora_adapter(const int32_t* __restrict__ offsets, int adapters, int64_t p, int64_t rows) {
-  int lo = 0, hi = adapters;   // offsets[lo] <= p (or lo = 0)
+  int lo = -1, hi = adapters;   // offsets[lo] <= p (or lo = -1)
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (lora_offset(offsets, mid, rows) <= p) lo = mid;
