@@ -478,6 +478,7 @@ gate_backward_kernel(T* d_logits, const float* __restrict__ d_weights, const flo
     if (ek == idx) mine += ak;   // (in turn, so all slots of an expert hold the same number)
   }
   T* out = d_logits + token * experts;
+  __syncwarp();   // (in place: a lane overwrites logits that another has read; shuffles promise no order of memory accesses)
 #pragma unroll
   for (int i = 0; i < COUNT; ++i) {
     const int e = (i * 32 + lane) * VEC;
