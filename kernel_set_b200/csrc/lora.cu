@@ -112,7 +112,7 @@ ks_status_t run_weight_grad(const char* where, const LoraWeightGrad& p, ks_dtype
   return KS_SUCCESS;
 }
 
-// What both directions ask of their sizes; *done with nothing to do.
+// What both directions ask of their sizes.
 ks_status_t check_sizes(const char* where, int64_t rows, int adapters, int rank, int64_t k, int64_t n, ks_dtype_t dtype) {
   const std::string w(where);
   if (rows < 0 || adapters <= 0 || rank <= 0 || k <= 0 || n <= 0) KSB_FAIL(KS_ERROR_INVALID_ARGUMENT, w + ": bad shape");
