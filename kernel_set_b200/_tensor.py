@@ -140,6 +140,14 @@ def same_dtype(reference: TensorLike, **others: TensorLike) -> None:
                 raise ValueError(f"{name} must be {reference.dtype}, as the other tensors of the call; got {t.dtype}")
 
 
+def same_device(reference: TensorLike, **others: TensorLike) -> None:
+    """Refuses CUDA tensors of another device than ``reference``'s: the kernels run there and would read addresses that are not its own."""
+    if isinstance(reference, torch.Tensor):
+        for name, t in others.items():
+            if isinstance(t, torch.Tensor) and t.is_cuda and t.device != reference.device:
+                raise ValueError(f"{name} must be on {reference.device}, as the other tensors of the call; got {t.device}")
+
+
 def at_least(numel: int, dtype: Optional[torch.dtype], **tensors: TensorLike) -> None:
     """Refuses tensors of fewer than ``numel`` elements or of another type (raw addresses have neither)."""
     for name, t in tensors.items():

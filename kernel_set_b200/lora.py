@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 
 from ._lib import by_address as lib, check
-from ._tensor import TensorLike, allocating_on, default_stream, dtype_to_ks, i32_ptr, on_device_of, ptr
+from ._tensor import TensorLike, allocating_on, default_stream, dtype_to_ks, i32_ptr, on_device_of, ptr, same_device
 
 
 def plan(adapter_ids: torch.Tensor, num_adapters: int, sorted_ids: Optional[torch.Tensor] = None,
@@ -31,6 +31,7 @@ def plan(adapter_ids: torch.Tensor, num_adapters: int, sorted_ids: Optional[torc
     for name, given in (("adapter_ids", adapter_ids), ("sorted_ids", sorted_ids), ("offsets", offsets)):
         if given is not None and given.dtype != torch.int32:
             raise ValueError(f"{name} must be int32; got {given.dtype}")
+    same_device(adapter_ids, sorted_ids=sorted_ids, offsets=offsets)
     tokens = adapter_ids.numel()
     if sorted_ids is None or offsets is None:
         with allocating_on(stream, adapter_ids.device):
@@ -80,6 +81,7 @@ def _refuse(rows: dict, flat: dict, sorted_ids, offsets, adapters: int) -> None:
     for name, (t, shape, dtype) in flat.items():
         ptr(t, name=name)
     ptr(offsets, name="offsets")
+    same_device(rows["x"][0], offsets=offsets, **{name: t for name, (t, shape, dtype) in {**rows, **flat}.items()})
     raise AssertionError("unreachable")
 
 
@@ -89,9 +91,9 @@ def _dims(x: torch.Tensor, b: torch.Tensor):
     return (*x.shape, *b.shape)
 
 
-def _plan_ok(sorted_ids, offsets, tokens: int, adapters: int) -> bool:
-    return (offsets.dtype is torch.int32 and offsets.is_cuda and offsets.is_contiguous() and offsets.numel() > adapters
-            and (sorted_ids is None or (sorted_ids.dtype is torch.int32 and sorted_ids.is_cuda and sorted_ids.is_contiguous()
+def _plan_ok(sorted_ids, offsets, tokens: int, adapters: int, dev: int) -> bool:
+    return (offsets.dtype is torch.int32 and offsets.get_device() == dev and offsets.is_contiguous() and offsets.numel() > adapters
+            and (sorted_ids is None or (sorted_ids.dtype is torch.int32 and sorted_ids.get_device() == dev and sorted_ids.is_contiguous()
                                         and sorted_ids.numel() == tokens)))
 
 
@@ -104,14 +106,14 @@ def apply(out: torch.Tensor, base: torch.Tensor, x: torch.Tensor, a: torch.Tenso
     so a slice of a fused projection's columns will do), ``a [adapters, rank, K]``, ``b [adapters, N, rank]``, all f16 or bf16;
     ``scales [adapters]`` fp32; ``h [tokens, rank]`` fp32 receives ``A x`` for :func:`backward`."""
     tokens, k, adapters, n, rank = _dims(x, b)
-    dt = x.dtype
+    dt, dev = x.dtype, x.get_device()
     # one quick test of everything: the smallest calls are bound by the host's path
     if not (out.shape == base.shape == (tokens, n) and a.shape == (adapters, rank, k) and scales.shape == (adapters,)
             and out.dtype is base.dtype is a.dtype is b.dtype is dt and scales.dtype is torch.float32
-            and out.is_cuda and base.is_cuda and x.is_cuda and a.is_cuda and b.is_cuda and scales.is_cuda
+            and out.get_device() == base.get_device() == a.get_device() == b.get_device() == scales.get_device() == dev >= 0
             and (ld_out := _ld(out, tokens, n)) >= 0 and (ld_base := _ld(base, tokens, n)) >= 0 and (ld_x := _ld(x, tokens, k)) >= 0
-            and a.is_contiguous() and b.is_contiguous() and scales.is_contiguous() and _plan_ok(sorted_ids, offsets, tokens, adapters)
-            and (h is None or (h.shape == (tokens, rank) and h.dtype is torch.float32 and h.is_cuda and h.is_contiguous()))):
+            and a.is_contiguous() and b.is_contiguous() and scales.is_contiguous() and _plan_ok(sorted_ids, offsets, tokens, adapters, dev)
+            and (h is None or (h.shape == (tokens, rank) and h.dtype is torch.float32 and h.get_device() == dev and h.is_contiguous()))):
         flat = {"a": (a, (adapters, rank, k), dt), "b": (b, (adapters, n, rank), dt), "scales": (scales, (adapters,), torch.float32)}
         if sorted_ids is not None:
             flat["sorted_ids"] = (sorted_ids, (tokens,), torch.int32)
@@ -147,17 +149,17 @@ def backward(d_x: torch.Tensor, d_a: torch.Tensor, d_b: torch.Tensor, d_x_base: 
     ``stream``'s pool) if not given.
     Returns ``(d_x, d_a, d_b)``."""
     tokens, k, adapters, n, rank = _dims(x, b)
-    dt = x.dtype
+    dt, dev = x.dtype, x.get_device()
     if not (d_x.shape == d_x_base.shape == (tokens, k) and d_out.shape == (tokens, n) and a.shape == d_a.shape == (adapters, rank, k)
             and d_b.shape == (adapters, n, rank) and h.shape == (tokens, rank) and scales.shape == (adapters,)
             and d_x.dtype is d_x_base.dtype is d_out.dtype is a.dtype is d_a.dtype is b.dtype is d_b.dtype is dt
             and h.dtype is scales.dtype is torch.float32
-            and d_x.is_cuda and d_x_base.is_cuda and d_out.is_cuda and x.is_cuda and a.is_cuda and d_a.is_cuda and b.is_cuda and d_b.is_cuda
-            and h.is_cuda and scales.is_cuda and a.is_contiguous() and d_a.is_contiguous() and b.is_contiguous() and d_b.is_contiguous()
+            and d_x.get_device() == d_x_base.get_device() == d_out.get_device() == a.get_device() == d_a.get_device() == b.get_device()
+            == d_b.get_device() == h.get_device() == scales.get_device() == dev >= 0 and a.is_contiguous() and d_a.is_contiguous() and b.is_contiguous() and d_b.is_contiguous()
             and h.is_contiguous() and scales.is_contiguous()
             and (ld_d_x := _ld(d_x, tokens, k)) >= 0 and (ld_d_x_base := _ld(d_x_base, tokens, k)) >= 0
             and (ld_d_out := _ld(d_out, tokens, n)) >= 0 and (ld_x := _ld(x, tokens, k)) >= 0
-            and _plan_ok(sorted_ids, offsets, tokens, adapters)):
+            and _plan_ok(sorted_ids, offsets, tokens, adapters, dev)):
         flat = {"a": (a, (adapters, rank, k), dt), "d_a": (d_a, (adapters, rank, k), dt), "b": (b, (adapters, n, rank), dt),
                 "d_b": (d_b, (adapters, n, rank), dt), "h": (h, (tokens, rank), torch.float32),
                 "scales": (scales, (adapters,), torch.float32)}
@@ -165,6 +167,7 @@ def backward(d_x: torch.Tensor, d_a: torch.Tensor, d_b: torch.Tensor, d_x_base: 
             flat["sorted_ids"] = (sorted_ids, (tokens,), torch.int32)
         _refuse({"d_x": (d_x, (tokens, k), dt), "d_x_base": (d_x_base, (tokens, k), dt), "d_out": (d_out, (tokens, n), dt),
                  "x": (x, (tokens, k), dt)}, flat, sorted_ids, offsets, adapters)
+    same_device(x, workspace=workspace)
     if workspace is None:
         with allocating_on(stream, x.device):   # (it goes back to that stream's pool when this returns: later calls there come behind)
             workspace = torch.empty(backward_workspace(tokens, adapters, rank, k, n), dtype=torch.uint8, device=x.device)

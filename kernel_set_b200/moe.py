@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from ._lib import by_address as lib, check
-from ._tensor import TensorLike, at_least, default_stream, dtype_to_ks, f32_ptr, i32_ptr, infer_dtype, on_device_of, ptr, same_dtype
+from ._tensor import TensorLike, at_least, default_stream, dtype_to_ks, f32_ptr, i32_ptr, infer_dtype, on_device_of, ptr, same_device, same_dtype
 
 
 def grouped_gemm(c: TensorLike, a: TensorLike, b: TensorLike, expert_offsets: TensorLike, num_experts: int,
@@ -129,8 +129,11 @@ def unpermute_backward(d_permuted: TensorLike, d_weights: TensorLike, d_out: Ten
             is torch.Tensor and d_permuted.dtype is d_out.dtype is permuted.dtype and d_weights.dtype is routing_weights.dtype is torch.float32
             and sorted_token_ids.dtype is torch.int32 and d_weights.numel() >= pairs and routing_weights.numel() >= pairs
             and sorted_token_ids.numel() >= pairs and d_permuted.numel() >= pairs * hidden and permuted.numel() >= pairs * hidden
-            and d_out.numel() >= num_tokens * hidden):
+            and d_out.numel() >= num_tokens * hidden and permuted.get_device() == d_permuted.get_device() == d_out.get_device()
+            == d_weights.get_device() == routing_weights.get_device() == sorted_token_ids.get_device()):
         same_dtype(permuted, d_permuted=d_permuted, d_out=d_out)
+        same_device(permuted, d_permuted=d_permuted, d_out=d_out, d_weights=d_weights, routing_weights=routing_weights,
+                    sorted_token_ids=sorted_token_ids)
         at_least(pairs, torch.float32, d_weights=d_weights, routing_weights=routing_weights)
         at_least(pairs, torch.int32, sorted_token_ids=sorted_token_ids)
         at_least(pairs * hidden, None, d_permuted=d_permuted, permuted=permuted)
@@ -152,8 +155,9 @@ def permute_backward(d_input: TensorLike, d_permuted: TensorLike, sorted_token_i
     pairs = num_tokens * top_k
     if not (type(d_input) is type(d_permuted) is type(sorted_token_ids) is torch.Tensor and d_input.dtype is d_permuted.dtype
             and sorted_token_ids.dtype is torch.int32 and sorted_token_ids.numel() >= pairs and d_permuted.numel() >= pairs * hidden
-            and d_input.numel() >= num_tokens * hidden):
+            and d_input.numel() >= num_tokens * hidden and d_permuted.get_device() == d_input.get_device() == sorted_token_ids.get_device()):
         same_dtype(d_permuted, d_input=d_input)
+        same_device(d_permuted, d_input=d_input, sorted_token_ids=sorted_token_ids)
         at_least(pairs, torch.int32, sorted_token_ids=sorted_token_ids)
         at_least(pairs * hidden, None, d_permuted=d_permuted)
         at_least(num_tokens * hidden, None, d_input=d_input)
@@ -174,8 +178,11 @@ def gate_softmax_topk_backward(d_logits: TensorLike, d_weights: TensorLike, weig
     if not (type(d_logits) is type(d_weights) is type(weights) is type(indices) is torch.Tensor
             and d_weights.dtype is weights.dtype is torch.float32 and indices.dtype is torch.int32 and d_weights.numel() >= pairs
             and weights.numel() >= pairs and indices.numel() >= pairs and d_logits.numel() >= numel
-            and (logits is None or (type(logits) is torch.Tensor and logits.dtype is d_logits.dtype and logits.numel() >= numel))):
+            and d_logits.get_device() == d_weights.get_device() == weights.get_device() == indices.get_device()
+            and (logits is None or (type(logits) is torch.Tensor and logits.dtype is d_logits.dtype and logits.numel() >= numel
+                                    and logits.get_device() == d_logits.get_device()))):
         same_dtype(d_logits, logits=logits)
+        same_device(d_logits, d_weights=d_weights, weights=weights, indices=indices, logits=logits)
         at_least(pairs, torch.float32, d_weights=d_weights, weights=weights)
         at_least(pairs, torch.int32, indices=indices)
         at_least(numel, None, d_logits=d_logits, logits=logits)
