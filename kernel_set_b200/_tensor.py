@@ -140,6 +140,14 @@ def same_dtype(reference: TensorLike, **others: TensorLike) -> None:
                 raise ValueError(f"{name} must be {reference.dtype}, as the other tensors of the call; got {t.dtype}")
 
 
+def of_dtype(dtype: Optional[int], **tensors: TensorLike) -> None:
+    """Refuses tensors whose type is not the one that the caller gave, if any: their memory would be read, and its end judged, as of that type."""
+    if dtype is not None:
+        for name, t in tensors.items():
+            if isinstance(t, torch.Tensor) and dtype_to_ks(t.dtype) != int(dtype):
+                raise ValueError(f"{name} must be {ks_to_torch_dtype(dtype)}, as dtype says; got {t.dtype}")
+
+
 def same_device(reference: TensorLike, **others: TensorLike) -> None:
     """Refuses CUDA tensors of another device than ``reference``'s: the kernels run there and would read addresses that are not its own."""
     if isinstance(reference, torch.Tensor):

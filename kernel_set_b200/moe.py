@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from ._lib import by_address as lib, check
-from ._tensor import TensorLike, at_least, default_stream, dtype_to_ks, f32_ptr, i32_ptr, infer_dtype, on_device_of, ptr, same_device, same_dtype
+from ._tensor import TensorLike, at_least, default_stream, dtype_to_ks, f32_ptr, i32_ptr, infer_dtype, of_dtype, on_device_of, ptr, same_device, same_dtype
 
 
 def grouped_gemm(c: TensorLike, a: TensorLike, b: TensorLike, expert_offsets: TensorLike, num_experts: int,
@@ -123,6 +123,7 @@ def unpermute_backward(d_permuted: TensorLike, d_weights: TensorLike, d_out: Ten
     ``d_weights[t,k] = <d_out[t], permuted[r]>`` (fp32). Rows without a pair and pairs without a row get zeros; a pair may
     occur once in ``sorted_token_ids``. ``d_permuted`` may be ``permuted``. Returns ``(d_permuted, d_weights)``."""
     dt = infer_dtype(permuted, dtype)
+    of_dtype(dtype, permuted=permuted, d_permuted=d_permuted, d_out=d_out)
     pairs = num_tokens * top_k
     # one quick test of types and sizes, the message where it fails
     if not (type(d_permuted) is type(permuted) is type(d_out) is type(d_weights) is type(routing_weights) is type(sorted_token_ids)
@@ -152,6 +153,7 @@ def permute_backward(d_input: TensorLike, d_permuted: TensorLike, sorted_token_i
     """Gradient of :func:`permute`: ``d_input[t]`` is the sum of token ``t``'s rows of ``d_permuted``, in slot order, in
     fp32; a pair may occur once in ``sorted_token_ids``."""
     dt = infer_dtype(d_permuted, dtype)
+    of_dtype(dtype, d_permuted=d_permuted, d_input=d_input)
     pairs = num_tokens * top_k
     if not (type(d_input) is type(d_permuted) is type(sorted_token_ids) is torch.Tensor and d_input.dtype is d_permuted.dtype
             and sorted_token_ids.dtype is torch.int32 and sorted_token_ids.numel() >= pairs and d_permuted.numel() >= pairs * hidden
@@ -174,6 +176,7 @@ def gate_softmax_topk_backward(d_logits: TensorLike, d_weights: TensorLike, weig
     """Gradient of :func:`gate_softmax_topk` with respect to the logits. ``weights`` and ``indices`` are what the gate
     gave; ``logits`` may be ``None`` with ``renormalize``. ``d_logits`` may be ``logits``."""
     dt = infer_dtype(d_logits, dtype)
+    of_dtype(dtype, d_logits=d_logits, logits=logits)
     pairs, numel = num_tokens * top_k, num_tokens * num_experts
     if not (type(d_logits) is type(d_weights) is type(weights) is type(indices) is torch.Tensor
             and d_weights.dtype is weights.dtype is torch.float32 and indices.dtype is torch.int32 and d_weights.numel() >= pairs

@@ -149,3 +149,18 @@ def test_plan_refuses_buffers_of_other_types_and_sizes(ks):
             ks.lora.plan(ids, 2, sorted_ids, offsets)
     with pytest.raises(ValueError, match="CUDA tensor"):
         ks.lora.plan(ids, 2, torch.zeros(6, dtype=torch.int32), torch.zeros(4, dtype=torch.int32))
+
+
+def test_moe_backward_wrappers_refuse_a_dtype_that_is_not_the_tensors(ks):
+    """A given dtype is for raw addresses; one wider than the tensors' would be read beyond their ends."""
+    bf, f, i = torch.bfloat16, torch.zeros(4, 2), torch.zeros(8, dtype=torch.int32)
+    rows, pairs = torch.zeros(4, 8, dtype=bf), torch.zeros(8, 8, dtype=bf)
+    for dtype, match in ((ks.DType.F32, "as dtype says"), (ks.DType.F16, "as dtype says"), (ks.DType.BF16, "CUDA tensor")):
+        with pytest.raises(ValueError, match=match):
+            ks.moe.unpermute_backward(pairs, f, rows, pairs, i, f, 4, 2, 8, dtype=dtype)
+        with pytest.raises(ValueError, match=match):
+            ks.moe.permute_backward(rows, pairs, i, 4, 2, 8, dtype=dtype)
+        with pytest.raises(ValueError, match=match):
+            ks.moe.gate_softmax_topk_backward(rows, f, f, i, rows, 4, 8, 2, dtype=dtype)
+    with pytest.raises(ValueError, match="as dtype says"):     # beside raw addresses too
+        ks.moe.permute_backward(4096, pairs, i, 4, 2, 8, dtype=ks.DType.F32)
