@@ -76,10 +76,12 @@ KS_API ks_status_t ks_lora_backward_workspace(size_t* bytes, int64_t num_tokens,
  *   d_a, d_b are written whole, with zeros for an adapter without rows
  *   workspace: 16-byte aligned device memory of the size above, undefined on entry and exit; two calls
  *   that may overlap need one each
- * d_out is the gradient of base as it is. g and h enter the products as A x does in ks_lora_apply; for d_a and d_b in f16
- * "largest" is the adapter's, and an adapter whose elements lie further apart than 2^33 gets plain fp32 sums, as do, in both types,
- * sums that are not finite (7.6 ms against 0.15 where that is all of d_b for 16384 rows of rank 64 beside 4096 x 4096). Sums in fp32, one rounding; the order of the
- * additions depends on the sizes only.
+ * d_out is the gradient of base as it is. Sums in fp32, one rounding. g and h enter the products as A x does in
+ * ks_lora_apply; for d_a and d_b in f16 "largest" is the adapter's, and an adapter whose elements lie further apart than
+ * 2^33 gets plain fp32 sums, as do, in both types, sums that are not finite (slow: 7.6 ms against 0.15 where that is all
+ * of d_b for 16384 rows of rank 64 beside 4096 x 4096). A row whose g is not finite gets NaN in d_x where it would get
+ * infinities. The same inputs and plan give the same bits; how the additions of d_a and d_b are grouped depends on the sizes
+ * and on the adapter's number of rows.
  */
 KS_API ks_status_t ks_lora_backward(
     void* d_x, int64_t ld_d_x, void* d_a, void* d_b, const void* d_x_base,

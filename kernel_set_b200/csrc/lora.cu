@@ -19,8 +19,9 @@ namespace {
 constexpr int kMaxAnyRank = 4096;
 constexpr int kAnyThreads = 256;
 // Rows up to which the forward pass takes 8 to 32 at a time instead of tiles of 128, by rank (us cold, few / tiles): rank 16, 512 rows of 64
-// adapters beside 4096 x 14336 42 / 67, of one beside 4096 x 4096 19.5 / 22.6; rank 32, 700 rows of 64 34 / 34, 1024 rows 38 / 34;
-// rank 64, 300 rows of 8 30 / 24, 512 of 64 44 / 38.
+// adapters beside 4096 x 14336 43 / 68, of one beside 4096 x 4096 18.5 / 22.5; rank 32, 700 rows of 64 33 / 35, 1024 rows 37 / 35;
+// rank 64, 256 rows of 64 35 / 39, 300 of 8 31 / 23, 512 of 64 43 / 39; rank 128, 200 of 8 35 / 27. Rows an adapter and widths move the
+// border, which the rule does not see: rank 16, 1000 rows of 300 adapters 74 / 92, of 4 of 64 27 / 31, of 64 beside 1024 x 1024 27 / 16.
 constexpr int few_rows(int rank) { return rank <= 32 ? 512 : 256; }
 
 // Any rank, widths and alignment: a CTA per place. The warps take the ranks in turn, a lane every 32nd product of a
