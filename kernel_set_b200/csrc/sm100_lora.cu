@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(TileCfg<RC>::kThreads, TileCfg<RC>::kPerSm) lo
           const uint64_t ad = umma_smem_desc_sw128(a + kk * 32, 16, 1024);
           const uint64_t bd = FWD ? umma_smem_desc_sw128(b + kk * 32, 16, 1024)
                                   : umma_smem_desc_sw128(b + kk * 16 * 128, kBlockBytes, 1024);
-          umma_f16_elect(tmem + (it & 1 ? C::kOdd : 0), ad, bd, q.idesc1, it + kk > 1 || kk == 1 ? 1u : 0u);
+          umma_f16_elect(tmem + (it & 1 ? C::kOdd : 0), ad, bd, q.idesc1, it > 1 || kk > 0 ? 1u : 0u);
         }
         tc_commit_elect(free1(s));
       }
